@@ -1,0 +1,595 @@
+// Paged key / value cache: appending new tokens' keys and values with their rotation, and attention of new tokens
+// over the cache.
+//
+// Row n of the new tokens belongs to sequence b with cu_q[b] <= n < cu_q[b + 1] and stands at cache position
+// kv_len[b] - (cu_q[b + 1] - cu_q[b]) + (n - cu_q[b]); position t lies in slot t % P of page block_table[b][t / P].
+// A page id outside [0, pages) names no page: nothing is written there and its keys are not seen, so no table
+// content can reach memory outside the pages.
+#include "pfm_serve.h"
+
+namespace {
+
+// Sequence of row n: how many sequences end at or before it, 64 at a time. All lanes of the wave take part and n is the
+// same in each of them. c.batch for rows behind the last sequence.
+__device__ __forceinline__ int seq_of_row(const PagedKv& c, int n, int lane) {
+    if (!c.cu_q) return n;
+    int b = 0;
+    for (int i0 = 0; i0 < c.batch; i0 += 64) {
+        const int i = i0 + lane;
+        const int ended = __popcll(__ballot(i < c.batch && c.cu_q[i + 1] <= n));
+        b += ended;
+        if (ended < 64) break;
+    }
+    return b;
+}
+
+__device__ __forceinline__ long long page_of(const PagedKv& c, int b, int t) {   // t inside the table's reach
+    const int pg = c.table[b * c.table_stride + t];
+    return pg >= 0 && pg < c.pages ? pg : -1;
+}
+
+template <typename T> struct Vec8 { T x[8]; };
+template <typename T> __device__ __forceinline__ Vec8<T> load8(const char* p) {
+    Vec8<T> v;
+#pragma unroll
+    for (int i = 0; i < (int)(8 * sizeof(T) / 16); ++i) ((float4*)&v)[i] = ((const float4*)p)[i];
+    return v;
+}
+template <typename T> __device__ __forceinline__ void store8(char* p, const Vec8<T>& v) {
+#pragma unroll
+    for (int i = 0; i < (int)(8 * sizeof(T) / 16); ++i) ((float4*)p)[i] = ((const float4*)&v)[i];
+}
+
+// ---- append -------------------------------------------------------------------------------------------------------
+// One workgroup per TB tokens. The angles pos * inv_freq are reduced to a turn in 64 bits (a far position's angle has
+// lost its fraction in 32), the sine and cosine are taken once per token and pair and shared by all heads through LDS.
+constexpr int AP_T = 256;
+
+template <typename T, int TB>
+__global__ __launch_bounds__(AP_T) void kv_append_kernel(AppendArgs a) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    __shared__ long long dst_page[TB];
+    __shared__ int dst_slot[TB];            // -1: the row has no sequence; -2: rotated, but no place to write
+    __shared__ int turn_pos[TB];
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+    const int half = a.inv_freq ? a.rot / 2 : 0;
+    float2* cs = (float2*)smem;             // [TB][half] (cos, sin)
+    const PagedKv& c = a.c;
+    const int n0 = blockIdx.x * TB;
+
+    for (int t = wid; t < TB; t += AP_T / 64) {
+        const int n = n0 + t;
+        int slot = -1, pos = 0;
+        long long page = 0;
+        if (n < c.tokens) {
+            const int b = seq_of_row(c, n, lane);
+            int first, end;
+            if (b < c.batch) {
+                c.rows(b, first, end);
+                if (n >= first) {
+                    const int len = c.len(b), at = len - (end - first) + (n - first);
+                    slot = -2;
+                    if (at >= 0 && at < len) {
+                        const int pi = c.by_page.div(at);
+                        page = page_of(c, b, pi);
+                        if (page >= 0) slot = at - pi * c.page;
+                    }
+                    pos = a.pos ? a.pos[n] : at;
+                }
+            }
+        }
+        if (lane == 0) { dst_page[t] = page; dst_slot[t] = slot; turn_pos[t] = pos; }
+    }
+    __syncthreads();
+    for (int i = tid; i < TB * half; i += AP_T) {
+        const int t = i / half, f = i - t * half;
+        if (dst_slot[t] != -1) {
+            double r = (double)turn_pos[t] * (double)a.inv_freq[f] * 0.15915494309189533577;   // turns
+            r -= rint(r);
+            float s, co;
+            sincospif((float)(2.0 * r), &s, &co);
+            cs[i] = make_float2(co, s);
+        }
+    }
+    __syncthreads();
+
+    // work items of a token: rotated pairs of 8-wide pieces, the unrotated rest of q and k, the pieces of v
+    const int D8 = c.dim / 8, h8 = half / 8, rest8 = D8 - 2 * h8;
+    const int turned = (a.q_heads + c.heads) * h8, kept = (a.q_heads + c.heads) * rest8, vals = c.heads * D8;
+    const int per = turned + kept + vals;
+    constexpr int E = sizeof(T);
+    for (int i = tid; i < TB * per; i += AP_T) {
+        const int t = i / per;
+        int w = i - t * per;
+        const int n = n0 + t, slot = dst_slot[t];
+        if (slot == -1) continue;
+        if (w < turned + kept) {
+            const bool turn = w < turned;
+            if (!turn) w -= turned;
+            const int per_h = turn ? h8 : rest8;
+            int h = w / per_h;
+            const int j = w - h * per_h;
+            const bool isq = h < a.q_heads;
+            const char* src;
+            char* dst;
+            if (isq) {
+                src = a.q.p + ((long long)n * a.q.ts + (long long)h * a.q.hs) * E;
+                dst = a.qo.p + ((long long)n * a.qo.ts + (long long)h * a.qo.hs) * E;
+            } else {
+                h -= a.q_heads;
+                if (slot < 0) continue;
+                src = a.k.p + ((long long)n * a.k.ts + (long long)h * a.k.hs) * E;
+                dst = c.k + (dst_page[t] * c.ks[0] + (long long)slot * c.ks[1] + (long long)h * c.ks[2]) * E;
+            }
+            if (!turn) {
+                const int o = (2 * h8 + j) * 8 * E;
+                store8<T>(dst + o, load8<T>(src + o));
+                continue;
+            }
+            // the two pieces of a pair group: (x1 | x2) half a rotated width apart, or 16 neighbours
+            const int o1 = a.interleaved ? j * 16 * E : j * 8 * E, o2 = a.interleaved ? o1 + 8 * E : o1 + half * E;
+            Vec8<T> p = load8<T>(src + o1), q = load8<T>(src + o2), p2, q2;
+            const float2* m = cs + t * half + j * 8;
+            if (a.interleaved) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 f = m[e], g = m[e + 4];
+                    const float x = to_f(p.x[2 * e]), y = to_f(p.x[2 * e + 1]), z = to_f(q.x[2 * e]), u = to_f(q.x[2 * e + 1]);
+                    p2.x[2 * e] = from_f<T>(x * f.x - y * f.y);
+                    p2.x[2 * e + 1] = from_f<T>(y * f.x + x * f.y);
+                    q2.x[2 * e] = from_f<T>(z * g.x - u * g.y);
+                    q2.x[2 * e + 1] = from_f<T>(u * g.x + z * g.y);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float2 f = m[e];
+                    const float x = to_f(p.x[e]), y = to_f(q.x[e]);
+                    p2.x[e] = from_f<T>(x * f.x - y * f.y);
+                    q2.x[e] = from_f<T>(y * f.x + x * f.y);
+                }
+            }
+            store8<T>(dst + o1, p2);
+            store8<T>(dst + o2, q2);
+        } else {
+            w -= turned + kept;
+            if (slot < 0) continue;
+            const int h = w / D8, o = (w - h * D8) * 8 * E;
+            store8<T>(c.v + (dst_page[t] * c.vs[0] + (long long)slot * c.vs[1] + (long long)h * c.vs[2]) * E + o,
+                      load8<T>(a.v.p + ((long long)n * a.v.ts + (long long)h * a.v.hs) * E + o));
+        }
+    }
+}
+
+// ---- attention ----------------------------------------------------------------------------------------------------
+// Operand traits. The products run swapped, S^T = K Q^T and O^T = V^T P^T: in both accumulators the query row is the
+// lane (lane & 15), so a row's maximum, sum and rescale are per lane, and the probabilities of two 16-key tiles are, as
+// they stand in S^T's registers, the second product's operand: its contraction index 8 g + j is key 4 g + j of the
+// first tile (j < 4) or key 4 g + j - 4 of the second, for the lane group g = lane >> 4.
+typedef short v4i16 __attribute__((ext_vector_type(4)));
+typedef short v8i16 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
+
+template <typename T> struct Mma;
+template <> struct Mma<bf16> {
+    typedef bf16x8 frag;
+    static __device__ __forceinline__ f32x4 mul(frag a, frag b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+};
+template <> struct Mma<f16> {
+    typedef f16x8 frag;
+    static __device__ __forceinline__ f32x4 mul(frag a, frag b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+};
+
+__device__ __forceinline__ float group_max(float x) {   // over the four lanes of a query row
+    x = fmaxf(x, __shfl_xor(x, 16, 64));
+    return fmaxf(x, __shfl_xor(x, 32, 64));
+}
+__device__ __forceinline__ float group_sum(float x) {
+    x += __shfl_xor(x, 16, 64);
+    return x + __shfl_xor(x, 32, 64);
+}
+template <typename T> __device__ __forceinline__ bool finite8(const Vec8<T>& v) {
+    bool ok = true;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ok = ok && (fabsf(to_f(v.x[i])) < INFINITY);
+    return ok;
+}
+
+constexpr int DEC_W = 4;      // waves of a workgroup; each runs over key blocks of its own
+constexpr int KB = 32;        // keys of a block
+template <typename T, int DP> struct DecGeom {
+    static constexpr int PITCH = DP * sizeof(T) + (sizeof(T) == 2 ? 32 : 16);   // rows of V: no bank met twice
+    static constexpr int VB = KB * PITCH;
+    static constexpr int OFF = KB * 8;                                          // the block's V row offsets
+    static constexpr int WAVE = VB + OFF;
+    static constexpr int MERGE = DEC_W * 16 * (DP + 4) * 4;                     // overlays the V blocks at the end
+    static constexpr int LDS = DEC_W * WAVE > MERGE ? DEC_W * WAVE : MERGE;
+};
+
+// Row tile x of all sequences, `rows` query rows (token, head of the group) each: its sequence and place there.
+// Every lane of every wave comes to the same answer.
+__device__ __forceinline__ bool find_tile(const PagedKv& c, int group, int rows, int x, int lane, int& b, int& tile) {
+    if (!c.cu_q) {
+        const int per = (group + rows - 1) / rows;
+        b = x / per;
+        tile = x - b * per;
+        return b < c.batch;
+    }
+    for (int i0 = 0; i0 < c.batch; i0 += 64) {
+        const int i = i0 + lane;
+        int tiles = 0;
+        if (i < c.batch) {
+            int first, end;
+            c.rows(i, first, end);
+            tiles = (int)(((long long)max(end - first, 0) * group + rows - 1) / rows);
+        }
+        int sum = tiles;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int s = __shfl_up(sum, o, 64);
+            if (lane >= o) sum += s;
+        }
+        const unsigned long long past = __ballot(sum > x);
+        if (past) {
+            const int l = __ffsll((long long)past) - 1;
+            b = i0 + l;
+            tile = x - __shfl(sum - tiles, l, 64);
+            return true;
+        }
+        x -= __shfl(sum, 63, 64);
+    }
+    return false;
+}
+
+// One workgroup = 16 query rows of one sequence and kv head; its waves take key blocks in turn, each with its own V
+// block in LDS and no barrier until the waves' results are joined.
+template <typename T, int DP>
+__global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a) {
+    using G = DecGeom<T, DP>;
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int ND = DP / 16;
+    constexpr int E = sizeof(T);
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    __shared__ float ml[DEC_W][16][2];
+    const PagedKv& c = a.c;
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+    const int r = lane & 15, g = lane >> 4;
+    const int hk = blockIdx.y;
+    int b, tile;
+    if (!find_tile(c, a.group, 16, blockIdx.x, lane, b, tile)) return;
+    int first, end;
+    c.rows(b, first, end);
+    const int nq = end - first, len = c.len(b);
+    const int rows = min(16, nq * a.group - tile * 16);            // of this tile
+    const int row = min(tile * 16 + r, nq * a.group - 1);
+    const int place = a.by_group.div(row);
+    const int head = hk * a.group + row - place * a.group;
+    const int pos = len - nq + place;
+    // keys the tile's rows see, as [lo, hi) of all and whether every row sees a whole block
+    const int pmin = len - nq + a.by_group.div(tile * 16), pmax = len - nq + a.by_group.div(tile * 16 + rows - 1);
+    const int hi = a.causal ? min(len, pmax + 1) : len;
+    const int lo = a.window ? max(0, pmin - a.window + 1) : 0;
+    const int blk0 = lo / KB, nblk = hi > lo ? (hi + KB - 1) / KB - blk0 : 0;
+    const int split = blockIdx.z;
+    const int s0 = (int)((long long)nblk * split / a.splits), s1 = (int)((long long)nblk * (split + 1) / a.splits);
+
+    unsigned char* Vs = smem + wid * G::WAVE;
+    long long* Vo = (long long*)(Vs + G::VB);
+
+    // Q in the operand layout: 16-bit: dims 32 c + 8 g ..; 32-bit: dims 16 c + 4 g .. (the same order as K below)
+    Vec8<T> qf[DP / 32];
+    {
+        const char* qp = a.q.p + ((long long)(first + place) * a.q.ts + (long long)head * a.q.hs) * E;
+#pragma unroll
+        for (int k = 0; k < DP / 32; ++k) {
+            const int d0 = F32 ? 32 * k + 4 * g : 32 * k + 8 * g;
+            qf[k] = Vec8<T>{};
+            if constexpr (F32) {
+                if (d0 < c.dim) ((float4*)&qf[k])[0] = *(const float4*)(qp + d0 * E);
+                if (d0 + 16 < c.dim) ((float4*)&qf[k])[1] = *(const float4*)(qp + (d0 + 16) * E);
+            } else if (d0 < c.dim) {
+                qf[k] = load8<T>(qp + d0 * E);
+            }
+        }
+    }
+    f32x4 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+
+    for (int blk = s0 + wid; blk < s1; blk += DEC_W) {
+        const int j0 = (blk0 + blk) * KB;
+        // the lane's key rows j0 + r and j0 + 16 + r; -1: no such key
+        long long ko[2];
+        bool here[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int j = j0 + 16 * t + r;
+            here[t] = j >= lo && j < hi;
+            long long vo = -1;
+            ko[t] = 0;
+            if (here[t]) {
+                const int pi = c.by_page.div(j), slot = j - pi * c.page;
+                const long long pg = page_of(c, b, pi);
+                here[t] = pg >= 0;
+                if (here[t]) {
+                    ko[t] = (pg * c.ks[0] + (long long)slot * c.ks[1] + (long long)hk * c.ks[2]) * E;
+                    vo = (pg * c.vs[0] + (long long)slot * c.vs[1] + (long long)hk * c.vs[2]) * E;
+                }
+            }
+            if (g == 0) Vo[16 * t + r] = vo;
+        }
+        __builtin_amdgcn_wave_barrier();
+        // keys this lane's scores belong to (rows 4 g + i of each tile) that exist
+        unsigned exist;
+        {
+            const unsigned e0 = (unsigned)(__ballot(here[0]) & 0xffff), e1 = (unsigned)(__ballot(here[1]) & 0xffff);
+            exist = ((e0 >> (4 * g)) & 15) | (((e1 >> (4 * g)) & 15) << 4);
+        }
+        // S^T = K Q^T
+        f32x4 s[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            Vec8<T> kf[DP / 32];
+#pragma unroll
+            for (int k = 0; k < DP / 32; ++k) {
+                const int d0 = F32 ? 32 * k + 4 * g : 32 * k + 8 * g;
+                kf[k] = Vec8<T>{};
+                if constexpr (F32) {
+                    if (here[t] && d0 < c.dim) ((float4*)&kf[k])[0] = *(const float4*)(c.k + ko[t] + d0 * E);
+                    if (here[t] && d0 + 16 < c.dim) ((float4*)&kf[k])[1] = *(const float4*)(c.k + ko[t] + (d0 + 16) * E);
+                } else if (here[t] && d0 < c.dim) {
+                    kf[k] = load8<T>(c.k + ko[t] + d0 * E);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < DP / 32; ++k) {
+                if constexpr (F32) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[k].x[e], qf[k].x[e], s[t], 0, 0, 0);
+                } else {
+                    s[t] = Mma<T>::mul(*(typename Mma<T>::frag*)&kf[k], *(typename Mma<T>::frag*)&qf[k], s[t]);
+                }
+            }
+        }
+        // V rows into LDS, absent ones as zeros
+        const bool edge = j0 < lo || j0 + KB > hi || (a.causal && j0 + KB - 1 > pmin) || (a.window && j0 <= pmax - a.window);
+        bool odd = false;     // a value that is not finite, in a block that some row sees in part
+        constexpr int CPR = DP / 8;      // 8-wide pieces of a row
+#pragma unroll
+        for (int i = 0; i < KB * CPR / 64; ++i) {
+            const int q8 = i * 64 + lane, kr = q8 / CPR, d0 = (q8 % CPR) * 8;
+            const long long vo = Vo[kr];
+            Vec8<T> v = Vec8<T>{};
+            if (vo >= 0 && d0 < c.dim) v = load8<T>(c.v + vo + d0 * E);
+            if (edge && !finite8(v)) {
+                odd = true;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (!(fabsf(to_f(v.x[e])) < INFINITY)) v.x[e] = from_f<T>(0.f);
+            }
+            store8<T>((char*)Vs + kr * G::PITCH + d0 * E, v);
+        }
+        // scores in base-2 exponents; a key that the row does not see is replaced, whatever its score is
+        unsigned seen = exist;
+        if (edge) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int j = j0 + 16 * (e >> 2) + 4 * g + (e & 3);
+                if ((a.causal && j > pos) || (a.window && j <= pos - a.window)) seen &= ~(1u << e);
+            }
+        }
+        float mt = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float x = s[e >> 2][e & 3] * a.scale_log2;
+            x = (seen >> e) & 1 ? x : -INFINITY;
+            s[e >> 2][e & 3] = x;
+            mt = fmaxf(mt, x);      // passes a NaN over: its own probability carries it on
+        }
+        mt = group_max(mt);
+        const float mn = fmaxf(m, mt), mu = mn == -INFINITY ? 0.f : mn;
+        const float corr = __builtin_amdgcn_exp2f(m - mu);
+        m = mn;
+        float p[8], ls = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            p[e] = __builtin_amdgcn_exp2f(s[e >> 2][e & 3] - mu);
+            ls += p[e];
+        }
+        l = l * corr + ls;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[d] *= corr;
+        // O^T += V^T P^T (the wave reads what it wrote itself: a wait, no barrier)
+        __builtin_amdgcn_wave_barrier();
+        if constexpr (F32) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float* vr = (const float*)(Vs + (16 * (e >> 2) + 4 * g + (e & 3)) * G::PITCH) + r;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[16 * d], p[e], o[d], 0, 0, 0);
+            }
+        } else {
+            Vec8<T> pb;      // probabilities rounded to the type: relative to each its half step, as the values are
+#pragma unroll
+            for (int e = 0; e < 8; ++e) pb.x[e] = from_f<T>(p[e]);
+            // transposing read: of 4 rows x 16 dims, lane r of the group gets dim r of the 4 rows
+            const unsigned char* vp = Vs + (4 * g + (r >> 2)) * G::PITCH + (r & 3) * 8;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                const v4i16 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vp + 32 * d));
+                const v4i16 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vp + 16 * G::PITCH + 32 * d));
+                const v8i16 va = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+                o[d] = Mma<T>::mul(*(const typename Mma<T>::frag*)&va, *(typename Mma<T>::frag*)&pb, o[d]);
+            }
+        }
+        // values that are not finite belong to the rows that see them only: 0 x inf in the product would reach the rest
+        if (edge && __any(odd)) {
+            for (int kr = 0; kr < KB; ++kr) {
+                const long long vo = Vo[kr];
+                if (vo < 0) continue;
+                const int e = 4 * (kr >> 4) + (kr & 3), from = r + 16 * ((kr >> 2) & 3);
+                float pk = 0.f;
+                unsigned sk = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i == e) { pk = __shfl(p[i], from, 64); sk = __shfl((int)(seen >> i) & 1, from, 64); }
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int dd = 16 * d + 4 * g + i;
+                        const float v = dd < c.dim ? to_f(((const T*)(c.v + vo))[dd]) : 0.f;
+                        if (sk && !(fabsf(v) < INFINITY)) o[d][i] += pk * v;
+                    }
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+
+    // join the waves: their maxima, then their sums scaled to the common one
+    l = group_sum(l);
+    if (g == 0) { ml[wid][r][0] = m; ml[wid][r][1] = l; }
+    __syncthreads();
+    float mm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < DEC_W; ++w) mm = fmaxf(mm, ml[w][r][0]);
+    const float sc = __builtin_amdgcn_exp2f(m - (mm == -INFINITY ? 0.f : mm));
+    float* os = (float*)smem + wid * 16 * (DP + 4);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+        f32x4 x = o[d] * sc;
+        *(f32x4*)(os + r * (DP + 4) + 16 * d + 4 * g) = x;
+    }
+    __syncthreads();
+    const float* ob = (const float*)smem;
+    for (int i = tid; i < 16 * (DP / 8); i += DEC_W * 64) {
+        const int rr = i / (DP / 8), d0 = (i % (DP / 8)) * 8;
+        if (rr >= rows || d0 >= c.dim) continue;
+        float x[8] = {};
+#pragma unroll
+        for (int w = 0; w < DEC_W; ++w)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] += ob[(w * 16 + rr) * (DP + 4) + d0 + e];
+        const int row2 = tile * 16 + rr, pl = a.by_group.div(row2);
+        const int hd = hk * a.group + row2 - pl * a.group, n = first + pl;
+        float lsum = 0.f, mr = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < DEC_W; ++w) mr = fmaxf(mr, ml[w][rr][0]);
+        const float mu = mr == -INFINITY ? 0.f : mr;
+#pragma unroll
+        for (int w = 0; w < DEC_W; ++w) lsum += ml[w][rr][1] * __builtin_amdgcn_exp2f(ml[w][rr][0] - mu);
+        if (a.splits == 1) {
+            const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+            Vec8<T> y;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y.x[e] = from_f<T>(lsum == 0.f ? 0.f : x[e] * inv);
+            store8<T>(a.o.p + ((long long)n * a.o.ts + (long long)hd * a.o.hs) * E + d0 * E, y);
+        } else {
+            const long long pr = (long long)split * c.tokens * a.q_heads + (long long)n * a.q_heads + hd;
+            float* dst = a.part + pr * c.dim + d0;
+            *(f32x4*)dst = f32x4{x[0], x[1], x[2], x[3]};
+            *(f32x4*)(dst + 4) = f32x4{x[4], x[5], x[6], x[7]};
+            if (d0 == 0) { a.part_ml[2 * pr] = mr; a.part_ml[2 * pr + 1] = lsum; }
+        }
+    }
+}
+
+// Joins the splits of a row: one wave per row, the sums scaled to the splits' common maximum, then divided once.
+template <typename T>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
+    const PagedKv& c = a.c;
+    const int lane = threadIdx.x & 63;
+    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), nrow = (long long)c.tokens * a.q_heads;
+    if (row >= nrow) return;
+    const int n = (int)(row / a.q_heads), head = (int)(row - (long long)n * a.q_heads);
+    const int b = seq_of_row(c, n, lane);
+    if (b >= c.batch) return;                 // a row behind the last sequence: left as it is
+    int first, end;
+    c.rows(b, first, end);
+    if (n < first) return;
+    float m = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[2 * (s * nrow + row)]);
+    const float mu = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int d0 = lane * 4;
+    for (int s = 0; s < a.splits; ++s) {
+        const long long pr = s * nrow + row;
+        const float w = __builtin_amdgcn_exp2f(a.part_ml[2 * pr] - mu);
+        l += a.part_ml[2 * pr + 1] * w;
+        if (d0 < c.dim) x += *(const f32x4*)(a.part + pr * c.dim + d0) * w;
+    }
+    if (d0 >= c.dim) return;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = from_f<T>(l == 0.f ? 0.f : x[e] * inv);
+    char* dst = a.o.p + ((long long)n * a.o.ts + (long long)head * a.o.hs + d0) * (int)sizeof(T);
+    if constexpr (sizeof(T) == 4) *(float4*)dst = *(const float4*)y;
+    else *(float2*)dst = *(const float2*)y;
+}
+
+template <typename T, int DP>
+hipError_t run_rows(const PagedAttnArgs& a, hipStream_t st) {
+    static_assert(DecGeom<T, DP>::LDS <= 150 * 1024, "LDS of a workgroup");
+    const PagedKv& c = a.c;
+    // each sequence has at most one row tile that is not full
+    const long long tiles = c.cu_q ? (long long)c.tokens * a.group / 16 + c.batch
+                                   : (long long)c.batch * ((a.group + 15) / 16);
+    hipError_t e = hipFuncSetAttribute((const void*)paged_rows_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                       DecGeom<T, DP>::LDS);
+    if (e != hipSuccess) return e;
+    paged_rows_kernel<T, DP><<<dim3((unsigned)tiles, c.heads, a.splits), DEC_W * 64, DecGeom<T, DP>::LDS, st>>>(a);
+    PFM_LAUNCH_CHECK();
+    if (a.splits > 1) {
+        const long long rows = (long long)c.tokens * a.q_heads;
+        paged_join_kernel<T><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(a);
+        PFM_LAUNCH_CHECK();
+    }
+    return hipSuccess;
+}
+template <typename T>
+hipError_t run_attention(const PagedAttnArgs& a, hipStream_t st) {
+    if (a.c.dim <= 64) return run_rows<T, 64>(a, st);
+    if (a.c.dim <= 128) return run_rows<T, 128>(a, st);
+    return run_rows<T, 256>(a, st);
+}
+
+template <typename T>
+hipError_t run_append(const AppendArgs& a, hipStream_t st) {
+    const int half = a.inv_freq ? a.rot / 2 : 0;
+    if (a.c.tokens <= 1024) {
+        kv_append_kernel<T, 1><<<a.c.tokens, AP_T, half * sizeof(float2), st>>>(a);
+    } else {
+        kv_append_kernel<T, 4><<<(a.c.tokens + 3) / 4, AP_T, 4 * half * sizeof(float2), st>>>(a);
+    }
+    PFM_LAUNCH_CHECK();
+    return hipSuccess;
+}
+
+}  // namespace
+
+int pfm_paged_attention_splits(int batch, int tokens, int q_heads, int kv_heads, long long max_kv) {
+    const long long tiles = (long long)tokens * (q_heads / kv_heads) / 16 + batch;
+    const long long want = (768 + tiles * kv_heads - 1) / (tiles * kv_heads);
+    const long long most = (max_kv + KB * DEC_W - 1) / (KB * DEC_W);
+    const long long s = want < most ? want : most;
+    return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+}
+hipError_t pfm_paged_attention(int dtype, const PagedAttnArgs& a, hipStream_t st) {
+    if (dtype == DT_F32) return run_attention<float>(a, st);
+    if (dtype == DT_BF16) return run_attention<bf16>(a, st);
+    return run_attention<f16>(a, st);
+}
+hipError_t pfm_kv_append(int dtype, const AppendArgs& a, hipStream_t st) {
+    if (dtype == DT_F32) return run_append<float>(a, st);
+    if (dtype == DT_BF16) return run_append<bf16>(a, st);
+    return run_append<f16>(a, st);
+}

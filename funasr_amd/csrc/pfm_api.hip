@@ -17,6 +17,7 @@
 
 #include "../../include/pfm.h"
 #include "pfm_common.h"
+#include "pfm_serve.h"
 #include "pfm_stream.h"
 
 // ---- kernel launchers (k_*.hip)
@@ -194,13 +195,14 @@ int pfm_fail(int code, const char* msg) { return fail(code, msg); }
 // address handed to a kernel faults the device instead of failing the call, so every entry point asks the runtime
 // what each operand is before it launches anything and refuses with PFM_E_ARG, naming the operand. Interior pointers
 // of an allocation (tensor slices) resolve to the allocation. `dev` < 0: the calling thread's current device.
-struct DevOp { const char* name; const void* p; };
-static int check_dev(const char* fn, int dev, std::initializer_list<DevOp> ops) {
+typedef PfmDevOp DevOp;
+static int check_dev(const char* fn, int dev, const DevOp* ops, int n) {
     if (dev < 0 && hipGetDevice(&dev) != hipSuccess) {
         (void)hipGetLastError();
         return fail(PFM_E_HIP, std::string(fn) + ": no current HIP device");
     }
-    for (const DevOp& o : ops) {
+    for (const DevOp* op = ops; op != ops + n; ++op) {
+        const DevOp& o = *op;
         if (!o.p) continue;   // optional operand not given (required ones are null-checked before this)
         hipPointerAttribute_t a{};
         const hipError_t e = hipPointerGetAttributes(&a, o.p);
@@ -216,6 +218,10 @@ static int check_dev(const char* fn, int dev, std::initializer_list<DevOp> ops) 
     }
     return PFM_OK;
 }
+static int check_dev(const char* fn, int dev, std::initializer_list<DevOp> ops) {
+    return check_dev(fn, dev, ops.begin(), (int)ops.size());
+}
+int pfm_check_dev_ops(const char* fn, const PfmDevOp* ops, int n) { return check_dev(fn, -1, ops, n); }
 #define CHECK_DEV(fn, dev, ...)                                 \
     do {                                                        \
         const int _rc = check_dev(fn, dev, {__VA_ARGS__});      \

@@ -1,0 +1,99 @@
+// Token-by-token decoding over a paged key / value cache: argument blocks shared by the kernels (k_paged.hip,
+// k_sample.hip) and their C entry points (pfm_serve.hip).
+#pragma once
+#include "pfm_common.h"
+
+typedef _Float16 f16;
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+template <> __device__ __forceinline__ float to_f<f16>(f16 x) { return (float)x; }
+template <> __device__ __forceinline__ f16 from_f<f16>(float x) { return (f16)x; }
+
+// dtype code of the serving entry points beside DT_F32 / DT_BF16 (include/pfm.h PFM_F16; 2 is DT_X3 inside)
+enum { DT_F16 = 3 };
+
+// An operand of a C entry point, for the check that it is device memory (pfm_api.hip).
+struct PfmDevOp { const char* name; const void* p; };
+
+// x / d for 0 <= x < 2^31 by one multiply: m = ceil(2^(32 + s) / d) with s = ceil(log2 d) gives the exact quotient
+// (m < 2^33; the part above 2^32 is added back as x itself, which cannot overflow 64 bits).
+struct FastDiv {
+    uint32_t mul, shift, d;
+    __device__ __forceinline__ int div(int x) const {
+        return d == 1 ? x : (int)(((unsigned long long)__umulhi((uint32_t)x, mul) + (uint32_t)x) >> shift);
+    }
+};
+static inline FastDiv fast_div(uint32_t d) {
+    FastDiv f{0, 0, d};
+    while (f.shift < 31 && (1u << f.shift) < d) ++f.shift;
+    f.mul = (uint32_t)((((1ull << f.shift) - d) << 32) / d + 1);
+    return f;
+}
+
+// A batch of sequences whose keys and values lie in pages. Strides count elements; the head dimension is contiguous.
+struct PagedKv {
+    char *k, *v;                        // pages
+    long long ks[3], vs[3];             // strides of page, slot in the page, head
+    long long pages;
+    const int* table;                   // [batch][table_stride]: page of key positions P i .. P i + P - 1
+    long long table_stride;
+    int width;                          // entries of a table row that may be read
+    int page, heads, dim, batch, tokens;
+    FastDiv by_page;
+    const int* kv_len;                  // [batch]: keys of the sequence, this call's new tokens included
+    const int* cu_q;                    // [batch + 1]: first row of each sequence's new tokens, or null: one token each
+
+    // The sequence's keys: never more than its table row can name.
+    __device__ __forceinline__ int len(int b) const {
+        const long long cap = (long long)width * page;
+        const int n = kv_len[b];
+        return n < 0 ? 0 : n > cap ? (int)cap : n;
+    }
+    // New rows [first, end) of sequence b, kept inside [0, tokens).
+    __device__ __forceinline__ void rows(int b, int& first, int& end) const {
+        if (!cu_q) { first = b; end = b + 1; return; }
+        first = max(cu_q[b], 0);
+        end = min(cu_q[b + 1], tokens);
+    }
+};
+struct Rows {                           // [tokens][heads][dim] with any token / head stride
+    char* p;
+    long long ts, hs;
+};
+
+struct AppendArgs {
+    PagedKv c;
+    Rows q, k, v, qo;
+    int q_heads;                        // 0: no queries to rotate
+    const float* inv_freq;              // [rot / 2] or null: nothing is rotated
+    int rot, interleaved;
+    const int* pos;                     // [tokens] rotation positions, or null: the cache positions
+};
+hipError_t pfm_kv_append(int dtype, const AppendArgs& a, hipStream_t st);
+
+struct PagedAttnArgs {
+    PagedKv c;
+    Rows q, o;
+    int q_heads, group;                 // group = q_heads / c.heads
+    FastDiv by_group;
+    float scale_log2;                   // scale * log2(e)
+    int causal, window;
+    int splits;                         // workgroups that share one row tile's keys
+    float* part;                        // splits > 1: [splits][tokens * q_heads] rows of dim sums, then max and sum
+    float* part_ml;
+};
+hipError_t pfm_paged_attention(int dtype, const PagedAttnArgs& a, hipStream_t st);
+int pfm_paged_attention_splits(int batch, int tokens, int q_heads, int kv_heads, long long max_kv);
+
+struct SampleArgs {
+    const void* x;                      // logits [batch][ld]
+    long long ld;
+    int batch, vocab;
+    const float *u, *temperature, *top_p, *min_p;   // [batch]; null: off
+    const int* top_k;
+    int* token;
+    float* prob;
+    void* ws;
+};
+long long pfm_sample_ws_bytes(int batch, int vocab);
+hipError_t pfm_sample(int dtype, const SampleArgs& a, hipStream_t st);

@@ -6,6 +6,7 @@ product — a missing library or device raises `PfmError`.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from typing import Dict, Optional
@@ -17,7 +18,7 @@ from .config import CTTransformerConfig, ParaformerConfig, SenseVoiceConfig
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("PFM_LIB", os.path.join(_HERE, "_lib", "libpfm_hip.so"))
 
-PFM_F32, PFM_BF16 = 0, 1
+PFM_F32, PFM_BF16, PFM_F16 = 0, 1, 3
 ARCH_PARAFORMER, ARCH_SENSEVOICE, ARCH_PUNC = 0, 1, 2
 MODE_EXACT, MODE_FAST = 0, 1
 MODES = {"exact": MODE_EXACT, "fp32": MODE_EXACT, "fast": MODE_FAST, "bf16": MODE_FAST}
@@ -29,6 +30,7 @@ ABI_SYMBOLS = ("pfm_config_default", "pfm_config_sensevoice", "pfm_create", "pfm
                "pfm_profile_read", "pfm_streams_create", "pfm_streams_reset", "pfm_stream_step", "pfm_stream_step_beam",
                "pfm_streams_destroy", "pfm_fbank_raw", "pfm_lfr_gather", "pfm_config_punc", "pfm_run_punc", "pfm_vad_config_default", "pfm_vad_create",
                "pfm_vad_set_weight", "pfm_vad_missing_weights", "pfm_vad_reset", "pfm_vad_run", "pfm_vad_destroy", "pfm_vad_fbank_raw", "pfm_vad_frame_energy", "pfm_run_punc_host",
+               "pfm_op_kv_append", "pfm_paged_attention_ws_bytes", "pfm_op_paged_attention", "pfm_sample_ws_size", "pfm_op_sample",
                "pfm_vad_opts_default", "pfm_vad_detector_create", "pfm_vad_detector_push", "pfm_vad_detector_destroy")
 
 
@@ -71,6 +73,20 @@ class PfmVadOpts(ctypes.Structure):
                                                "noise_frame_num_used_for_snr", "frame_in_ms")] + \
               [(n, ctypes.c_double) for n in ("speech_2_noise_ratio", "snr_thres", "decibel_thres",
                                               "speech_noise_thres", "fe_prior_thres")]
+
+
+class PfmPagedKv(ctypes.Structure):
+    """pfm_paged_kv: the pages of a key / value cache, the tables and lengths of one batch."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_stride", ctypes.c_int64 * 3),
+                ("v_stride", ctypes.c_int64 * 3), ("pages", ctypes.c_int64), ("block_table", ctypes.c_void_p),
+                ("table_stride", ctypes.c_int64), ("kv_len", ctypes.c_void_p), ("cu_q", ctypes.c_void_p)] + \
+               [(n, ctypes.c_int32) for n in ("dtype", "table_width", "page_size", "heads", "head_dim", "batch",
+                                              "tokens")]
+
+
+class PfmRows(ctypes.Structure):
+    """pfm_rows: [tokens][heads][head_dim] at any token and head stride."""
+    _fields_ = [("p", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
 
 
 _lib = None
@@ -163,6 +179,14 @@ def load_library(path: Optional[str] = None) -> ctypes.CDLL:
     lib.pfm_vad_destroy.restype = None
     lib.pfm_streams_destroy.argtypes = [vp]
     lib.pfm_streams_destroy.restype = None
+    kvp, rows, i64 = ctypes.POINTER(PfmPagedKv), ctypes.POINTER(PfmRows), ctypes.c_int64
+    lib.pfm_op_kv_append.argtypes = [vp, kvp, rows, rows, rows, rows, i32, f32p, i32, i32, i32p]
+    lib.pfm_paged_attention_ws_bytes.argtypes = [kvp, i32]
+    lib.pfm_paged_attention_ws_bytes.restype = i64
+    lib.pfm_op_paged_attention.argtypes = [vp, kvp, rows, rows, i32, ctypes.c_float, i32, i32, vp, i64]
+    lib.pfm_sample_ws_size.argtypes = [i32, i32]
+    lib.pfm_sample_ws_size.restype = i64
+    lib.pfm_op_sample.argtypes = [vp, i32, vp, i64, i32, i32, f32p, f32p, i32p, f32p, f32p, i32p, f32p, vp, i64]
     for name in ABI_SYMBOLS:
         getattr(lib, name)
     if path is None:
@@ -180,6 +204,16 @@ def _ptr(t) -> Optional[int]:
     if t is None:
         return None
     return t.data_ptr()
+
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _on_device(torch, device):
+    """The call's device as the current one, where it is another (the library launches on the current device)."""
+    if device.type != "cuda":
+        raise PfmError(f"device tensors expected, got {device}")
+    return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _stream_ptr(torch, device) -> int:
@@ -772,6 +806,136 @@ def op_ctc_beam(am, x, lens, ntok, beam, ctc_weight, penalty=0.0, nbest=1, sos=1
                               int(sos), int(eos), int(blank), _ptr(tokens), L_cap, _ptr(nt), _ptr(sc)),
           "pfm_op_ctc_beam")
     return tokens, nt, sc
+
+
+# ---- token-by-token decoding over a paged key / value cache ---------------------------------
+def _serve_dtype(torch, t, what: str) -> int:
+    d = {torch.float32: PFM_F32, torch.bfloat16: PFM_BF16, torch.float16: PFM_F16}.get(t.dtype)
+    if d is None:
+        raise PfmError(f"{what}: float32, bfloat16 or float16 expected, got {t.dtype}")
+    return d
+
+
+def _vector(torch, t, n: int, dtype, device, what: str):
+    if t is not None and (t.dtype != dtype or t.shape != (n,) or t.device != device or (n > 1 and t.stride(0) != 1)):
+        raise PfmError(f"{what} must be a contiguous [{n}] {dtype} tensor on {device}, got {tuple(t.shape)} {t.dtype} "
+                       f"on {t.device}")
+    return t
+
+
+def _rows(t, n: int, heads: int, dim: int, dtype, device, what: str) -> PfmRows:
+    if t.shape != (n, heads, dim) or t.dtype != dtype or t.device != device:
+        raise PfmError(f"{what} must be [{n}, {heads}, {dim}] {dtype} on {device}, got {tuple(t.shape)} {t.dtype} on "
+                       f"{t.device}")
+    st = t.stride()
+    if st[2] != 1 and dim > 1:
+        raise PfmError(f"{what}: the head dimension must be contiguous")
+    return PfmRows(t.data_ptr(), st[0], st[1])
+
+
+def _paged_kv(torch, k_pages, v_pages, block_table, kv_len, cu_q, n: int) -> PfmPagedKv:
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
+        raise PfmError("k_pages and v_pages must be [pages, page_size, heads, head_dim] of one shape and type")
+    dt, dev = _serve_dtype(torch, k_pages, "k_pages"), k_pages.device
+    ks, vs = k_pages.stride(), v_pages.stride()
+    if ks[3] != 1 or vs[3] != 1 or v_pages.device != dev:
+        raise PfmError("k_pages and v_pages: one device and a contiguous head dimension expected")
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.device != dev or \
+            (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise PfmError(f"block_table must be [batch, width] int32 on {dev} with contiguous rows")
+    B, W = block_table.shape
+    _vector(torch, kv_len, B, torch.int32, dev, "kv_len")
+    _vector(torch, cu_q, B + 1, torch.int32, dev, "cu_q")
+    if cu_q is None and n != B:
+        raise PfmError(f"without cu_q every sequence has one new token: {n} rows for {B} sequences")
+    P, page, heads, dim = k_pages.shape
+    return PfmPagedKv(k_pages.data_ptr(), v_pages.data_ptr(), ks[:3], vs[:3], P, block_table.data_ptr(),
+                      block_table.stride(0) if B > 1 else W, kv_len.data_ptr(), _ptr(cu_q), dt, W, page, heads, dim, B, n)
+
+
+def op_kv_append(k, v, k_pages, v_pages, block_table, kv_len, cu_q=None, q=None, inv_freq=None, interleaved=False,
+                 pos=None, q_out=None):
+    """Append the new tokens' k, v [N, heads, D] to the paged cache k_pages, v_pages [pages, page_size, heads, D]
+    (written in place), rotating k, and q [N, q_heads, D] into the returned q_out, by pos * inv_freq
+    (pfm_op_kv_append). block_table [B, width], kv_len [B] (the new tokens included), cu_q [B + 1] (None: one token per
+    sequence), pos [N] (None: the cache positions): int32; inv_freq [rot_dim / 2] f32 (None: no rotation)."""
+    import torch
+    lib = load_library()
+    n, dev = k.shape[0], k_pages.device
+    kv = _paged_kv(torch, k_pages, v_pages, block_table, kv_len, cu_q, n)
+    rk = _rows(k, n, kv.heads, kv.head_dim, k_pages.dtype, dev, "k")
+    rv = _rows(v, n, kv.heads, kv.head_dim, k_pages.dtype, dev, "v")
+    rq = ro = None
+    hq = 0
+    if q is not None:
+        if q.dim() != 3:
+            raise PfmError("q must be [tokens, q_heads, head_dim]")
+        hq = q.shape[1]
+        rq = _rows(q, n, hq, kv.head_dim, k_pages.dtype, dev, "q")
+        if q_out is None:
+            q_out = torch.empty((n, hq, kv.head_dim), dtype=q.dtype, device=dev)
+        ro = _rows(q_out, n, hq, kv.head_dim, k_pages.dtype, dev, "q_out")
+    elif q_out is not None:
+        raise PfmError("q_out given without q")
+    if inv_freq is not None:
+        if inv_freq.dim() != 1:
+            raise PfmError("inv_freq must be [rot_dim / 2]")
+        _vector(torch, inv_freq, inv_freq.shape[0], torch.float32, dev, "inv_freq")
+    _vector(torch, pos, n, torch.int32, dev, "pos")
+    with _on_device(torch, dev):
+        check(lib.pfm_op_kv_append(_stream_ptr(torch, dev), kv, rk, rv, rq, ro, hq, _ptr(inv_freq),
+                                   0 if inv_freq is None else 2 * inv_freq.shape[0], 1 if interleaved else 0,
+                                   _ptr(pos)), "pfm_op_kv_append")
+    return q_out
+
+
+def op_paged_attention(q, k_pages, v_pages, block_table, kv_len, cu_q=None, scale=None, causal=True, window=0,
+                       out=None):
+    """Attention of the new tokens' q [N, q_heads, D] over the paged cache (pfm_op_paged_attention) -> out
+    [N, q_heads, D] in q's type. Query i of a sequence sees the keys j < kv_len with j <= i's position if causal and
+    j > i's position - window if window > 0; one that sees none gives zeros. scale: None = D ** -0.5."""
+    import torch
+    lib = load_library()
+    if q.dim() != 3:
+        raise PfmError("q must be [tokens, q_heads, head_dim]")
+    n, hq, dev = q.shape[0], q.shape[1], k_pages.device
+    kv = _paged_kv(torch, k_pages, v_pages, block_table, kv_len, cu_q, n)
+    rq = _rows(q, n, hq, kv.head_dim, k_pages.dtype, dev, "q")
+    if out is None:
+        out = torch.empty((n, hq, kv.head_dim), dtype=q.dtype, device=dev)
+    ro = _rows(out, n, hq, kv.head_dim, k_pages.dtype, dev, "out")
+    nb = lib.pfm_paged_attention_ws_bytes(kv, hq)
+    ws = torch.empty((nb,), dtype=torch.uint8, device=dev) if nb else None
+    with _on_device(torch, dev):
+        check(lib.pfm_op_paged_attention(_stream_ptr(torch, dev), kv, rq, ro, hq,
+                                         kv.head_dim ** -0.5 if scale is None else float(scale), 1 if causal else 0,
+                                         int(window), _ptr(ws), nb), "pfm_op_paged_attention")
+    return out
+
+
+def op_sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
+    """One token per row of logits [B, V] from the uniform numbers u [B] f32 (pfm_op_sample) -> (token [B] int32,
+    prob [B] f32, its probability among the kept tokens). Settings per row, None = off: temperature f32 (<= 0: the
+    largest logit), top_k int32 (<= 0: off), top_p f32 (>= 1: off), min_p f32 (<= 0: off)."""
+    import torch
+    lib = load_library()
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise PfmError("logits must be [B, V] with contiguous rows")
+    dt, dev, (B, V) = _serve_dtype(torch, logits, "logits"), logits.device, logits.shape
+    if u is None:
+        raise PfmError("u, one uniform number per row, is needed")
+    for t, d, what in ((u, torch.float32, "u"), (temperature, torch.float32, "temperature"),
+                       (top_k, torch.int32, "top_k"), (top_p, torch.float32, "top_p"), (min_p, torch.float32, "min_p")):
+        _vector(torch, t, B, d, dev, what)
+    token = torch.empty((B,), dtype=torch.int32, device=dev)
+    prob = torch.empty((B,), dtype=torch.float32, device=dev)
+    nb = lib.pfm_sample_ws_size(B, V)
+    ws = torch.empty((nb,), dtype=torch.uint8, device=dev) if nb else None
+    with _on_device(torch, dev):
+        check(lib.pfm_op_sample(_stream_ptr(torch, dev), dt, _ptr(logits), logits.stride(0) if B > 1 else V, B, V, _ptr(u),
+                                _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(token), _ptr(prob),
+                                _ptr(ws), nb), "pfm_op_sample")
+    return token, prob
 
 
 class PfmVad:

@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define PFM_ABI_VERSION 5
+#define PFM_ABI_VERSION 6
 
 enum pfm_status {
     PFM_OK = 0,
@@ -39,7 +39,7 @@ enum pfm_status {
                             arrival barrier timed out): the outputs of the call are not valid */
 };
 
-enum pfm_dtype { PFM_F32 = 0, PFM_BF16 = 1 };
+enum pfm_dtype { PFM_F32 = 0, PFM_BF16 = 1, PFM_F16 = 3 /* the paged-cache and sampling entry points */ };
 
 /* Numerics mode of pfm_run.
  *  EXACT: every GEMM and the attention as split-bf16 x6 MFMA (each f32 operand split into
@@ -462,6 +462,78 @@ int pfm_op_ctc_beam(void* stream, const float* am, int L, const float* x, int T,
                     const int32_t* ntok, int B, int V, int beam, float ctc_weight, float penalty, int nbest,
                     int end_detect, int sos, int eos, int blank, int32_t* tokens, int L_cap, int32_t* ntok_out,
                     float* scores_out);
+
+/* ---- token-by-token decoding over a paged key / value cache ----
+ * What an autoregressive text decoder does per step next to its matrix products: append the new tokens' keys and
+ * values (rotated by position) to the cache, attend over the cache, draw the next token. No handle: all memory is the
+ * caller's device memory, every call is one chain of launches on `stream`, without host synchronisation, allocation
+ * or memset, so it can be captured into a HIP graph and replayed with other lengths, tables and settings in the same
+ * buffers. Types: PFM_F32, PFM_BF16, PFM_F16; softmax statistics, sums and rotations are held in 32 bits or more.
+ *
+ * Sequence b of a batch keeps position t of its keys and values in slot t % page_size of page
+ * block_table[b][t / page_size]. Its new tokens are rows cu_q[b] .. cu_q[b + 1] - 1 of q / k / v (cu_q == NULL: row b,
+ * one token per sequence) and stand at the positions kv_len[b] - (their number) .. kv_len[b] - 1: kv_len counts the
+ * sequence's keys WITH this call's new tokens, for the append and the attention alike.
+ *  - Pages are [pages][page_size][heads][head_dim] in any order of the first three dimensions: k_stride / v_stride are
+ *    the strides of page, slot and head in elements; head_dim is contiguous, pointers are aligned to 16 bytes and
+ *    strides are multiples of 16 bytes.
+ *  - A table entry outside [0, pages) names no page: appends to it are dropped, its keys are not seen. kv_len is cut to
+ *    [0, table_width * page_size]. Entries behind the last position are not read.
+ *  - Rows of q / k / v at or behind cu_q[batch] belong to no sequence: their outputs are left as they were.
+ *  - Sequences may share pages that are only read. A page that is appended to belongs to one sequence: what two tokens
+ *    appended to one slot in the same call leave there is unspecified. */
+typedef struct pfm_paged_kv {
+    void* k;
+    void* v;
+    int64_t k_stride[3], v_stride[3];
+    int64_t pages;
+    const int32_t* block_table;   /* [batch][table_stride] */
+    int64_t table_stride;
+    const int32_t* kv_len;        /* [batch] */
+    const int32_t* cu_q;          /* [batch + 1], ascending from 0, or NULL */
+    int32_t dtype, table_width, page_size, heads, head_dim /* multiple of 8, at most 256 */, batch,
+        tokens /* rows of q / k / v */;
+} pfm_paged_kv;
+
+/* Rows [tokens][heads][head_dim] at any token and head stride (elements), e.g. a slice of a fused q|k|v projection. */
+typedef struct pfm_rows {
+    void* p;
+    int64_t token_stride, head_stride;
+} pfm_rows;
+
+/* Append k and v (heads of the cache) of the new tokens. With inv_freq [rot_dim / 2] (f32 device) the first rot_dim
+ * (multiple of 16) dims of every k head, and of every q head into q_out, are rotated by the angles
+ * pos * inv_freq[i]: (x1, x2) -> (x1 cos - x2 sin, x2 cos + x1 sin) for x1 = x[i], x2 = x[i + rot_dim / 2], or
+ * x[2 i], x[2 i + 1] with interleaved != 0. pos [tokens] int32 device or NULL: the cache positions. q_heads 0 (q, q_out
+ * NULL): keys only. q_out may be q itself with the same strides; without inv_freq q is copied. */
+int pfm_op_kv_append(void* stream, const pfm_paged_kv* cache, const pfm_rows* k, const pfm_rows* v, const pfm_rows* q,
+                     const pfm_rows* q_out, int q_heads, const float* inv_freq, int rot_dim, int interleaved,
+                     const int32_t* pos);
+
+/* out = softmax(scale q k^T) v over the cached keys, q_heads a multiple of the cache's heads (query head h reads cache
+ * head h / (q_heads / heads)). The query at position i sees the keys j < kv_len[b] with j <= i where causal != 0 and
+ * j > i - window where window > 0; a query that sees no key, or none with a score above -inf, gives zeros. Values of
+ * keys that a query does not see do not reach it, NaN and infinities included. ws: pfm_paged_attention_ws_bytes bytes
+ * of device memory (NULL if 0), free again when the call's work is done. */
+int64_t pfm_paged_attention_ws_bytes(const pfm_paged_kv* cache, int q_heads);
+int pfm_op_paged_attention(void* stream, const pfm_paged_kv* cache, const pfm_rows* q, const pfm_rows* out, int q_heads,
+                           float scale, int causal, int window, void* ws, int64_t ws_bytes);
+
+/* Draw one token per row of logits [B][ld] (V <= 2^20 used) from given uniform numbers u [B] f32 in [0, 1). Settings
+ * [B] device, NULL = off for every row: temperature f32 (<= 0: the largest logit; under 1e-30
+ * as 1e-30), top_k int32 (<= 0: off), top_p f32
+ * (>= 1: off), min_p f32 (<= 0: off). p = softmax(logits / temperature); tokens in the order of their logits, ties by
+ * index; kept are the first top_k, of these the ones before which less than top_p of their mass lies (the first in any
+ * case), of these the ones with p >= min_p max(p).
+ *   token [B] int32 out: the first kept index, in the vocabulary's order, whose running sum of p exceeds u times the
+ *         kept mass; -1 for a row without a logit above -inf. NaN logits are never drawn; +inf logits share the mass.
+ *   prob  [B] f32 out or NULL: its probability among the kept tokens.
+ * p is computed in 64 bits and summed in whole multiples of 2^-43 of the largest, so the result depends neither on
+ * the order of summation nor on the batch. ws: pfm_sample_ws_size bytes of device memory (NULL if 0). */
+int64_t pfm_sample_ws_size(int B, int V);
+int pfm_op_sample(void* stream, int dtype, const void* logits, int64_t ld, int B, int V, const float* u,
+                  const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                  int32_t* token, float* prob, void* ws, int64_t ws_bytes);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,185 @@
+"""Refusals of the paged-cache and sampling entry points, on the host: the C argument checks (before any device is
+asked for) and the Python wrappers' shape, type and device checks; and the oracle of the GPU tests against itself."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from funasr_amd import runtime as rt
+from oracle import serve_ref as ref
+
+P16 = 0x10000   # an aligned address that no check may read
+E_ARG = -1
+
+
+def cache(**kw):
+    c = rt.PfmPagedKv()
+    c.k, c.v, c.pages, c.page_size, c.heads, c.head_dim, c.dtype = P16, P16, 4, 16, 2, 64, rt.PFM_BF16
+    c.k_stride[:], c.v_stride[:] = (2048, 128, 64), (2048, 128, 64)
+    c.block_table, c.table_stride, c.table_width, c.kv_len, c.cu_q, c.batch, c.tokens = P16, 3, 3, P16, P16, 2, 5
+    for k, v in kw.items():
+        if k in ("k_stride", "v_stride"):
+            getattr(c, k)[:] = v
+        else:
+            setattr(c, k, v)
+    return c
+
+
+def rows(p=P16, ts=256, hs=64):
+    return rt.PfmRows(p, ts, hs)
+
+
+BAD_CACHE = [dict(dtype=2), dict(dtype=9), dict(batch=-1), dict(tokens=-1), dict(pages=-1), dict(table_width=-1),
+             dict(page_size=0), dict(heads=0), dict(heads=70000), dict(head_dim=0), dict(head_dim=60), dict(head_dim=264),
+             dict(k=None), dict(v=None), dict(block_table=None), dict(kv_len=None), dict(cu_q=None), dict(table_stride=2),
+             dict(k=P16 + 8), dict(v=P16 + 2), dict(k_stride=(2048, 128, 60)), dict(v_stride=(2044, 128, 64)),
+             dict(k_stride=(-2048, 128, 64)), dict(page_size=1 << 30, table_width=3)]
+
+
+@pytest.mark.parametrize("kw", BAD_CACHE, ids=str)
+def test_bad_cache_refused(kw):
+    lib = rt.load_library()
+    c = cache(**kw)
+    assert lib.pfm_op_kv_append(None, c, rows(), rows(), rows(), rows(), 4, None, 0, 0, None) == E_ARG
+    assert b"pfm_op_kv_append" in lib.pfm_last_error()
+    assert lib.pfm_op_paged_attention(None, c, rows(), rows(), 4, 1.0, 1, 0, P16, 1 << 40) == E_ARG
+    assert b"pfm_op_paged_attention" in lib.pfm_last_error()
+
+
+@pytest.mark.parametrize("k,v,q,qo,hq,freq,rot", [
+    (None, rows(), rows(), rows(), 4, P16, 64), (rows(), None, rows(), rows(), 4, P16, 64),
+    (rows(), rows(), None, rows(), 4, P16, 64), (rows(), rows(), rows(), None, 4, P16, 64),
+    (rows(P16 + 4), rows(), rows(), rows(), 4, P16, 64), (rows(ts=250), rows(), rows(), rows(), 4, P16, 64),
+    (rows(hs=-64), rows(), rows(), rows(), 4, P16, 64), (rows(), rows(), rows(), rows(hs=0), 4, P16, 64),
+    (rows(), rows(), rows(), rows(ts=0), 4, P16, 64), (rows(), rows(), rows(), rows(), -1, P16, 64),
+    (rows(), rows(), rows(), rows(), 4, P16, 8), (rows(), rows(), rows(), rows(), 4, P16, 24),
+    (rows(), rows(), rows(), rows(), 4, P16, 80)])
+def test_bad_append_refused(k, v, q, qo, hq, freq, rot):
+    lib = rt.load_library()
+    assert lib.pfm_op_kv_append(None, cache(), k, v, q, qo, hq, freq, rot, 0, None) == E_ARG
+
+
+@pytest.mark.parametrize("kw", [dict(k_stride=(0, 128, 64)), dict(v_stride=(2048, 128, 0)), dict(k_stride=(2048, 0, 64))])
+def test_append_to_overlapping_pages_refused(kw):
+    lib = rt.load_library()
+    assert lib.pfm_op_kv_append(None, cache(**kw), rows(), rows(), rows(), rows(), 4, None, 0, 0, None) == E_ARG
+
+
+@pytest.mark.parametrize("q,out,hq,scale,window,ws,nb", [
+    (None, rows(), 4, 1.0, 0, P16, 1 << 40), (rows(), None, 4, 1.0, 0, P16, 1 << 40),
+    (rows(), rows(), 3, 1.0, 0, P16, 1 << 40), (rows(), rows(), 0, 1.0, 0, P16, 1 << 40),
+    (rows(), rows(), 4, math.nan, 0, P16, 1 << 40), (rows(), rows(), 4, math.inf, 0, P16, 1 << 40),
+    (rows(), rows(), 4, 1.0, -1, P16, 1 << 40), (rows(P16 + 2), rows(), 4, 1.0, 0, P16, 1 << 40),
+    (rows(), rows(ts=0), 4, 1.0, 0, P16, 1 << 40), (rows(), rows(hs=0), 4, 1.0, 0, P16, 1 << 40)])
+def test_bad_attention_refused(q, out, hq, scale, window, ws, nb):
+    lib = rt.load_library()
+    assert lib.pfm_op_paged_attention(None, cache(), q, out, hq, scale, 1, window, ws, nb) == E_ARG
+
+
+def test_attention_workspace_refused():
+    lib = rt.load_library()
+    c = cache(table_width=4096, table_stride=4096, tokens=2)   # long caches, few rows: the keys are split
+    need = lib.pfm_paged_attention_ws_bytes(c, 4)
+    assert need > 0
+    for ws, nb in ((None, need), (P16, need - 1), (P16 + 4, need)):
+        assert lib.pfm_op_paged_attention(None, c, rows(), rows(), 4, 1.0, 1, 0, ws, nb) == E_ARG
+        assert b"pace" in lib.pfm_last_error()
+    assert lib.pfm_paged_attention_ws_bytes(None, 4) == 0
+    assert lib.pfm_paged_attention_ws_bytes(cache(batch=0, tokens=0), 4) == 0
+
+
+@pytest.mark.parametrize("kw", [dict(dtype=2), dict(B=-1), dict(V=0), dict(V=(1 << 20) + 1, ld=1 << 21), dict(ld=9),
+                                dict(logits=None), dict(u=None), dict(token=None), dict(logits=P16 + 1)], ids=str)
+def test_bad_sample_refused(kw):
+    lib = rt.load_library()
+    a = dict(dtype=rt.PFM_F32, logits=P16, ld=10, B=2, V=10, u=P16, token=P16) | kw
+    assert lib.pfm_op_sample(None, a["dtype"], a["logits"], a["ld"], a["B"], a["V"], a["u"], None, None, None, None,
+                             a["token"], None, P16, 1 << 40) == E_ARG
+    assert b"pfm_op_sample" in lib.pfm_last_error()
+
+
+def test_empty_batches_are_nothing():
+    lib = rt.load_library()
+    c = cache(batch=0, tokens=0)
+    assert lib.pfm_op_kv_append(None, c, None, None, None, None, 0, None, 0, 0, None) == 0
+    assert lib.pfm_op_paged_attention(None, c, None, None, 4, 1.0, 1, 0, None, 0) == 0
+    assert lib.pfm_op_sample(None, rt.PFM_F32, None, 10, 0, 10, None, None, None, None, None, None, None, None, 0) == 0
+
+
+def _args(N=3, B=3, W=2, P=8, page=4, hk=2, hq=4, D=16, dt=torch.float32):
+    return dict(k=torch.zeros(N, hk, D, dtype=dt), v=torch.zeros(N, hk, D, dtype=dt), q=torch.zeros(N, hq, D, dtype=dt),
+                kp=torch.zeros(P, page, hk, D, dtype=dt), vp=torch.zeros(P, page, hk, D, dtype=dt),
+                table=torch.zeros(B, W, dtype=torch.int32), kv_len=torch.ones(B, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("change", [
+    dict(k=torch.zeros(3, 2, 8)), dict(k=torch.zeros(2, 2, 16)), dict(k=torch.zeros(3, 2, 16).half()),
+    dict(v=torch.zeros(3, 1, 16)), dict(q=torch.zeros(3, 4, 8)), dict(q=torch.zeros(4, 4, 16)), dict(q=torch.zeros(3, 64)),
+    dict(kp=torch.zeros(8, 4, 32)), dict(vp=torch.zeros(8, 4, 2, 16).half()), dict(vp=torch.zeros(7, 4, 2, 16)),
+    dict(kp=torch.zeros(8, 4, 2, 16).double(), vp=torch.zeros(8, 4, 2, 16).double()),
+    dict(kp=torch.zeros(8, 4, 16, 2).transpose(2, 3), vp=torch.zeros(8, 4, 2, 16)),
+    dict(table=torch.zeros(3, 2)), dict(table=torch.zeros(3, dtype=torch.int32)),
+    dict(table=torch.zeros(2, 3, dtype=torch.int32).t()), dict(kv_len=torch.ones(3)),
+    dict(kv_len=torch.ones(4, dtype=torch.int32)), dict(table=torch.zeros(2, 2, dtype=torch.int32), kv_len=torch.ones(2, dtype=torch.int32)),
+    dict(cu_q=torch.zeros(3, dtype=torch.int32)), dict(cu_q=torch.zeros(4))], ids=lambda c: "-".join(f"{k}{tuple(v.shape)}" for k, v in c.items()))
+def test_wrappers_refuse(change):
+    a = _args() | change
+    cu = a.get("cu_q")
+    with pytest.raises(rt.PfmError):
+        rt.op_kv_append(a["k"], a["v"], a["kp"], a["vp"], a["table"], a["kv_len"], cu, q=a["q"])
+    if not {"k", "v"} & set(change):
+        with pytest.raises(rt.PfmError):
+            rt.op_paged_attention(a["q"], a["kp"], a["vp"], a["table"], a["kv_len"], cu)
+
+
+def test_wrappers_refuse_host_tensors_and_extras():
+    a = _args()
+    with pytest.raises(rt.PfmError):
+        rt.op_paged_attention(a["q"], a["kp"], a["vp"], a["table"], a["kv_len"])
+    with pytest.raises(rt.PfmError):
+        rt.op_kv_append(a["k"], a["v"], a["kp"], a["vp"], a["table"], a["kv_len"], q_out=a["q"])
+    for bad in (torch.zeros(2, 8), torch.zeros(8).double()):
+        with pytest.raises(rt.PfmError):
+            rt.op_kv_append(a["k"], a["v"], a["kp"], a["vp"], a["table"], a["kv_len"], inv_freq=bad)
+    x, u = torch.zeros(2, 10), torch.zeros(2)
+    for call in (lambda: rt.op_sample(x, u), lambda: rt.op_sample(x.double(), u), lambda: rt.op_sample(x[0], u),
+                 lambda: rt.op_sample(x.t(), torch.zeros(10)), lambda: rt.op_sample(x, None),
+                 lambda: rt.op_sample(x, u.double()), lambda: rt.op_sample(x, u, top_k=u),
+                 lambda: rt.op_sample(x, u, temperature=torch.zeros(3)), lambda: rt.op_sample(x, torch.zeros(4)[::2])):
+        with pytest.raises(rt.PfmError):
+            call()
+
+
+def test_struct_layout_matches_header():
+    """ctypes layouts against the C compiler's, by the header's field order and sizes."""
+    assert ctypes.sizeof(rt.PfmRows) == 24 and ctypes.sizeof(rt.PfmPagedKv) == 8 * 13 + 4 * 7 + 4
+    assert rt.PfmPagedKv.dtype.offset == 104 and rt.PfmPagedKv.tokens.offset == 128
+
+
+# ---- the oracle itself
+def test_oracle_sample_by_hand():
+    x = torch.log(torch.tensor([[0.1, 0.4, 0.2, 0.3]]))
+    s = lambda u, **kw: ref.sample(x, torch.tensor([u]), **kw)  # noqa: E731
+    assert s(0.05)[0] == [0] and s(0.3)[0] == [1] and s(0.6)[0] == [2] and s(0.99)[0] == [3]
+    assert s(0.0, top_k=torch.tensor([2]))[0] == [1] and s(0.99, top_k=torch.tensor([2]))[0] == [3]
+    t, p = s(0.99, top_p=torch.tensor([0.69]))
+    assert t == [3] and p[0] == pytest.approx(0.3 / 0.7, rel=1e-6)
+    assert s(0.0, min_p=torch.tensor([0.7]))[0] == [1]
+    assert s(0.9, temperature=torch.tensor([0.0]))[0] == [1]
+    assert ref.sample(torch.full((1, 3), -math.inf), torch.tensor([0.5])) == ([-1], [0.0])
+
+
+def test_oracle_attend_and_append_by_hand():
+    kp = torch.zeros(3, 2, 1, 8, dtype=torch.float64)
+    vp = torch.zeros_like(kp)
+    table = torch.tensor([[2, 0]], dtype=torch.int32)
+    k = torch.arange(24.0).view(3, 1, 8)
+    _, kp, vp = ref.append(k, 2 * k, kp, vp, table, torch.tensor([3]), torch.tensor([0, 3]))
+    assert torch.equal(kp[2, 0, 0], k[0, 0].double()) and torch.equal(vp[0, 0, 0], 2 * k[2, 0].double())
+    q = torch.zeros(3, 2, 8)
+    o, _, _ = ref.attend(q, kp, vp, table, torch.tensor([3]), torch.tensor([0, 3]))
+    assert torch.allclose(o[:, 0], torch.stack([2 * k[: i + 1, 0].double().mean(0) for i in range(3)]))
+    r = ref.rotate(torch.ones(1, 16, dtype=torch.float64), 1, torch.tensor([math.pi / 2] * 8), False)
+    assert torch.allclose(r, torch.tensor([[-1.0] * 8 + [1.0] * 8], dtype=torch.float64), atol=1e-6)
