@@ -5,6 +5,9 @@
 // kv_len[b] - (cu_q[b + 1] - cu_q[b]) + (n - cu_q[b]); position t lies in slot t % P of page block_table[b][t / P].
 // A page id outside [0, pages) names no page: nothing is written there and its keys are not seen, so no table
 // content can reach memory outside the pages.
+#include <algorithm>
+#include <type_traits>
+
 #include "pfm_serve.h"
 
 namespace {
@@ -29,6 +32,7 @@ __device__ __forceinline__ long long page_of(const PagedKv& c, int b, int t) {  
 }
 
 template <typename T> struct Vec8 { T x[8]; };
+template <typename T> struct Pack16 { T x[16 / sizeof(T)]; };
 template <typename T> __device__ __forceinline__ Vec8<T> load8(const char* p) {
     Vec8<T> v;
 #pragma unroll
@@ -199,6 +203,32 @@ template <typename T> __device__ __forceinline__ bool finite8(const Vec8<T>& v) 
     return ok;
 }
 
+// A scale's sign goes to the queries, and a scale of 0 as well (the scores' scale is 1 then): what is hidden stays at -inf.
+template <typename T> __device__ __forceinline__ T times(T x, int sign) { return from_f<T>(to_f(x) * (float)sign); }
+
+// a 32-bit word of values with zeros for those that are not finite; bad: there were such
+template <typename T> __device__ __forceinline__ float finite_word(float x, bool& bad) {
+    constexpr uint32_t M = sizeof(T) == 4 ? 0x7f800000u : std::is_same<T, f16>::value ? 0x7c00u : 0x7f80u;   // exponent
+    const uint32_t w = __float_as_uint(x);
+    uint32_t clear = (w & M) == M ? (sizeof(T) == 4 ? ~0u : 0xffffu) : 0u;
+    if (sizeof(T) == 2) clear |= ((w >> 16) & M) == M ? 0xffff0000u : 0u;
+    bad = bad || clear;
+    return __uint_as_float(w & ~clear);
+}
+
+// o[i ..] += the values that are not finite among the four dims dd .. of a value row
+template <typename T, typename V>
+__device__ __forceinline__ void add_odd(const T* row, int dd, int dim, V& o, int i) {
+    if (dd >= dim) return;
+    struct alignas(4 * sizeof(T)) Four { T x[4]; };
+    const Four v = *(const Four*)(row + dd);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float x = to_f(v.x[k]);
+        if (!(fabsf(x) < INFINITY)) o[i + k] += x;
+    }
+}
+
 constexpr int DEC_W = 4;      // waves of a workgroup; each runs over key blocks of its own
 constexpr int KB = 32;        // keys of a block
 template <typename T, int DP> struct DecGeom {
@@ -210,9 +240,10 @@ template <typename T, int DP> struct DecGeom {
     static constexpr int LDS = DEC_W * WAVE > MERGE ? DEC_W * WAVE : MERGE;
 };
 
-// Row tile x of all sequences, `rows` query rows (token, head of the group) each: its sequence and place there.
-// Every lane of every wave comes to the same answer.
-__device__ __forceinline__ bool find_tile(const PagedKv& c, int group, int rows, int x, int lane, int& b, int& tile) {
+// Row tile x, `rows` query rows (token, head of the group) each, of the sequences that have more than `over` and at most
+// `upto` rows: its sequence and place there. Every lane of every wave comes to the same answer.
+__device__ __forceinline__ bool find_tile(const PagedKv& c, int group, int rows, int over, int upto, int x, int lane,
+                                          int& b, int& tile) {
     if (!c.cu_q) {
         const int per = (group + rows - 1) / rows;
         b = x / per;
@@ -225,7 +256,8 @@ __device__ __forceinline__ bool find_tile(const PagedKv& c, int group, int rows,
         if (i < c.batch) {
             int first, end;
             c.rows(i, first, end);
-            tiles = (int)(((long long)max(end - first, 0) * group + rows - 1) / rows);
+            const int n = max(end - first, 0) * group;
+            tiles = n > over && n <= upto ? (n + rows - 1) / rows : 0;
         }
         int sum = tiles;
 #pragma unroll
@@ -258,9 +290,9 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
     const PagedKv& c = a.c;
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
     const int r = lane & 15, g = lane >> 4;
-    const int hk = blockIdx.y;
+    const int hk = blockIdx.x % c.heads;
     int b, tile;
-    if (!find_tile(c, a.group, 16, blockIdx.x, lane, b, tile)) return;
+    if (!find_tile(c, a.group, 16, 0, a.rows_upto, blockIdx.x / c.heads, lane, b, tile)) return;
     int first, end;
     c.rows(b, first, end);
     const int nq = end - first, len = c.len(b);
@@ -274,7 +306,7 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
     const int hi = a.causal ? min(len, pmax + 1) : len;
     const int lo = a.window ? max(0, pmin - a.window + 1) : 0;
     const int blk0 = lo / KB, nblk = hi > lo ? (hi + KB - 1) / KB - blk0 : 0;
-    const int split = blockIdx.z;
+    const int split = blockIdx.y;
     const int s0 = (int)((long long)nblk * split / a.splits), s1 = (int)((long long)nblk * (split + 1) / a.splits);
 
     unsigned char* Vs = smem + wid * G::WAVE;
@@ -294,6 +326,12 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
             } else if (d0 < c.dim) {
                 qf[k] = load8<T>(qp + d0 * E);
             }
+        }
+        if (a.q_sign != 1) {
+#pragma unroll
+            for (int k = 0; k < DP / 32; ++k)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) qf[k].x[e] = times(qf[k].x[e], a.q_sign);
         }
     }
     f32x4 o[ND];
@@ -429,25 +467,18 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
                 o[d] = Mma<T>::mul(*(const typename Mma<T>::frag*)&va, *(typename Mma<T>::frag*)&pb, o[d]);
             }
         }
-        // values that are not finite belong to the rows that see them only: 0 x inf in the product would reach the rest
+        // values that are not finite belong to the rows that see them only (whatever their weight): 0 x inf in the product
+        // would reach the rest
         if (edge && __any(odd)) {
             for (int kr = 0; kr < KB; ++kr) {
                 const long long vo = Vo[kr];
                 if (vo < 0) continue;
-                const int e = 4 * (kr >> 4) + (kr & 3), from = r + 16 * ((kr >> 2) & 3);
-                float pk = 0.f;
-                unsigned sk = 0;
+                const int j = j0 + kr;
+                if ((a.causal && j > pos) || (a.window && j <= pos - a.window)) continue;
+                int d0 = 4 * g;
+                asm volatile("" : "+v"(d0));       // nothing of this is kept ready for every block
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (i == e) { pk = __shfl(p[i], from, 64); sk = __shfl((int)(seen >> i) & 1, from, 64); }
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int dd = 16 * d + 4 * g + i;
-                        const float v = dd < c.dim ? to_f(((const T*)(c.v + vo))[dd]) : 0.f;
-                        if (sk && !(fabsf(v) < INFINITY)) o[d][i] += pk * v;
-                    }
+                for (int d = 0; d < ND; ++d) add_odd<T>((const T*)(c.v + vo), d0 + 16 * d, c.dim, o[d], 0);
             }
         }
         __builtin_amdgcn_wave_barrier();
@@ -501,6 +532,321 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
     }
 }
 
+// ---- chunks: row tiles that share their keys through LDS
+// The same swapped products on 32 x 32 tiles: a wave owns 32 query rows (row = lane & 31, h = lane >> 5), register e of
+// a score tile is key kappa(e) + 4 h, and registers 8 s .. 8 s + 7 are the probabilities of the second product's s-th
+// 16 keys in the order key 16 s + 4 h + j, 16 s + 8 + 4 h + j - 4.
+__device__ __forceinline__ int kappa(int e) { return (e & 3) + 8 * (e >> 2); }
+__device__ __forceinline__ float xor32_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float xor32_add(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+template <typename T> struct Mma32;
+template <> struct Mma32<bf16> {
+    static __device__ __forceinline__ f32x16 mul(bf16x8 a, bf16x8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+};
+template <> struct Mma32<f16> {
+    static __device__ __forceinline__ f32x16 mul(f16x8 a, f16x8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+};
+
+template <typename T, int DP> struct TileGeom {
+    static constexpr int E = sizeof(T);
+    static constexpr int NW = DP > 128 ? 4 : 8;            // waves: 256 registers each suffice up to 128 dims
+    static constexpr int ROWS = NW * 32;
+    static constexpr int KT = E == 2 && DP <= 128 ? 64 : 32;   // keys of a tile
+    static constexpr int CPR = DP * E / 16;                // 16-byte pieces of a row
+    static constexpr int KPITCH = E == 2 ? DP * 2 : DP * 4 + 16;
+    static constexpr int VPITCH = E == 2 ? DP * 2 + 64 : DP * 4;
+    static constexpr int STAGE = KT * (KPITCH + VPITCH);
+    static constexpr int LDS = 2 * STAGE;
+    static constexpr int PER = KT * CPR / (NW * 64);       // pieces of K, and of V, that a thread brings
+    // place of piece c of key row r: the 16 rows that a read of one piece column touches lie in different banks
+    static __device__ __forceinline__ int kpiece(int r, int c) {
+        if (E == 4) return c;
+        return CPR == 8 ? c ^ ((r >> 1) & 7) : c ^ (r & 15);
+    }
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__((TileGeom<T, DP>::NW * 64), (TileGeom<T, DP>::NW / 4)) void paged_tile_kernel(PagedAttnArgs a) {
+    using G = TileGeom<T, DP>;
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int E = sizeof(T), KT = G::KT, NB = KT / 32, ND = DP / 32, NT = G::NW * 64;
+    constexpr int NQ = DP * E / 32;                          // 16-byte pieces of a query row that a lane holds
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    __shared__ unsigned char there[2][KT];                   // the tile's keys that exist
+    __shared__ int odd[2];                                   // the last tile of a buffer with a value that is not finite
+    const PagedKv& c = a.c;
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, fr = lane & 31, h = lane >> 5;
+    const int hk = blockIdx.x % c.heads;
+    int b, tile;
+    if (!find_tile(c, a.group, G::ROWS, a.rows_upto, 0x7fffffff, (gridDim.x - 1 - blockIdx.x) / c.heads, lane, b, tile)) return;
+    int first, end;
+    c.rows(b, first, end);
+    const int nq = end - first, len = c.len(b), nrows = nq * a.group, base = len - nq;
+    const int row0 = tile * G::ROWS, row1 = min(row0 + G::ROWS, nrows) - 1;
+    const int pmin = base + a.by_group.div(row0), pmax = base + a.by_group.div(row1);
+    // this wave's rows; -1 rows: none
+    const int w0 = row0 + wid * 32, w1 = min(w0 + 32, nrows) - 1;
+    const bool idle = w0 >= nrows;
+    const int wmin = idle ? 0 : base + a.by_group.div(w0), wmax = idle ? -1 : base + a.by_group.div(w1);
+    const int row = min(w0 + fr, nrows - 1), place = a.by_group.div(row), head = hk * a.group + row - place * a.group;
+    const int pos = base + place;
+    const int hi = a.causal ? min(len, pmax + 1) : len;
+    const int lo = a.window ? max(0, pmin - a.window + 1) : 0;
+    const int tile0 = lo / KT, ntile = hi > lo ? (hi + KT - 1) / KT - tile0 : 0;
+    const int split = blockIdx.y;
+    const int t0 = tile0 + (int)((long long)ntile * split / a.tile_splits);
+    const int t1 = tile0 + (int)((long long)ntile * (split + 1) / a.tile_splits);
+
+    float4 qf[NQ];   // 16-bit: dims 16 k + 8 h ..; 32-bit: dims 8 k + 4 h ..
+    {
+        const char* qp = a.q.p + ((long long)(first + place) * a.q.ts + (long long)head * a.q.hs) * E + 16 * h;
+#pragma unroll
+        for (int k = 0; k < NQ; ++k)
+            qf[k] = (2 * k + h) * 16 < c.dim * E ? *(const float4*)(qp + 32 * k) : make_float4(0.f, 0.f, 0.f, 0.f);
+        if (a.q_sign != 1) {
+#pragma unroll
+            for (int k = 0; k < NQ; ++k) {
+                Pack16<T> x = *(Pack16<T>*)&qf[k];
+#pragma unroll
+                for (int e = 0; e < 16 / E; ++e) x.x[e] = times(x.x[e], a.q_sign);
+                qf[k] = *(float4*)&x;
+            }
+        }
+    }
+    f32x16 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+    float m = -INFINITY, l = 0.f;
+
+    // staging: the thread's pieces are column tid % CPR of the rows tid / CPR + i NT / CPR
+    constexpr int PER = G::PER, RSTEP = NT / G::CPR;
+    const int scol = tid % G::CPR, srow = tid / G::CPR;
+    const bool in_dim = scol * 16 < c.dim * E;
+    int page[PER];
+    auto pages = [&](int t) {          // page ids of tile t's rows; -1: no such key
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int j = t * KT + srow + i * RSTEP;
+            page[i] = -1;
+            if (j >= lo && j < hi) page[i] = c.table[b * c.table_stride + c.by_page.div(j)];
+            if ((unsigned long long)(long long)page[i] >= (unsigned long long)c.pages) page[i] = -1;
+        }
+    };
+    struct Stage { float4 k[PER], v[PER]; };
+    const char* kb0 = c.k + ((long long)hk * c.ks[2]) * E + scol * 16;
+    const char* vb0 = c.v + ((long long)hk * c.vs[2]) * E + scol * 16;
+    auto fetch = [&](int t) -> Stage {
+        Stage s;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int j = t * KT + srow + i * RSTEP, slot = j - c.by_page.div(j) * c.page;
+            s.k[i] = s.v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (page[i] >= 0 && in_dim) {
+                s.k[i] = *(const float4*)(kb0 + ((long long)page[i] * c.ks[0] + (long long)slot * c.ks[1]) * E);
+                s.v[i] = *(const float4*)(vb0 + ((long long)page[i] * c.vs[0] + (long long)slot * c.vs[1]) * E);
+            }
+        }
+        return s;
+    };
+    auto put = [&](int t, Stage& s, const int (&pg)[PER]) {
+        unsigned char* K = smem + (t & 1) * G::STAGE;
+        unsigned char* V = K + KT * G::KPITCH;
+        // a tile that some row of the workgroup sees in part: values that are not finite are set aside
+        const bool part = (a.causal && t * KT + KT - 1 > pmin) || (a.window && t * KT <= pmax - a.window);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int r = srow + i * RSTEP;
+            if (scol == 0) there[t & 1][r] = pg[i] >= 0;
+            if (part) {
+                bool bad = false;
+                s.v[i] = make_float4(finite_word<T>(s.v[i].x, bad), finite_word<T>(s.v[i].y, bad),
+                                     finite_word<T>(s.v[i].z, bad), finite_word<T>(s.v[i].w, bad));
+                if (bad) odd[t & 1] = t;
+            }
+            *(float4*)(K + r * G::KPITCH + G::kpiece(r, scol) * 16) = s.k[i];
+            *(float4*)(V + r * G::VPITCH + scol * 16) = s.v[i];
+        }
+    };
+    const int tr_row = 4 * h + ((lane & 15) >> 2), tr_col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+
+    auto compute = [&](int t) {
+        const unsigned char* K = smem + (t & 1) * G::STAGE;
+        const unsigned char* V = K + KT * G::KPITCH;
+        const int j0 = t * KT;
+        f32x16 s[NB];
+#pragma unroll
+        for (int kb = 0; kb < NB; ++kb) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
+            const int r = kb * 32 + fr;
+#pragma unroll
+            for (int k = 0; k < NQ; ++k) {
+                const float4 kf = *(const float4*)(K + r * G::KPITCH + G::kpiece(r, 2 * k + h) * 16);
+                if constexpr (F32) {
+                    s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.x, qf[k].x, s[kb], 0, 0, 0);
+                    s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.y, qf[k].y, s[kb], 0, 0, 0);
+                    s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.z, qf[k].z, s[kb], 0, 0, 0);
+                    s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.w, qf[k].w, s[kb], 0, 0, 0);
+                } else {
+                    s[kb] = Mma32<T>::mul(*(const typename Mma<T>::frag*)&kf, *(const typename Mma<T>::frag*)&qf[k], s[kb]);
+                }
+            }
+        }
+        const unsigned long long here = __ballot(lane < KT && there[t & 1][lane & (KT - 1)]);
+        const bool some = here != (KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1);
+        const bool edge = some || (a.causal && j0 + KT - 1 > wmin) || (a.window && j0 <= wmax - a.window);
+        if (edge) {
+            asm volatile("" ::: "memory");    // a branch of its own: not folded into every tile
+#pragma unroll
+            for (int kb = 0; kb < NB; ++kb) {
+                // bit k: the row sees key j1 + k
+                const int j1 = j0 + kb * 32 + 4 * h;
+                unsigned bits = (unsigned)(here >> (32 * kb)) >> (4 * h);
+                if (a.causal) bits &= pos - j1 >= 31 ? ~0u : pos < j1 ? 0u : (2u << (pos - j1)) - 1;
+                if (a.window) {
+                    const int n = pos - a.window + 1 - j1;       // so many keys of them are too far back
+                    bits &= n <= 0 ? ~0u : n > 31 ? 0u : ~0u << n;
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[kb][e] = bits & (1u << kappa(e)) ? s[kb][e] : -INFINITY;
+            }
+        }
+        // m is the maximum at its last change, in units of the products: a score may pass it by 2^8 before all is rescaled
+        float mt = -INFINITY;
+#pragma unroll
+        for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[kb][e]);
+        mt = xor32_max(mt) * a.scale_log2;
+        if (__any(mt > m + 8.f)) {
+            const float mn = fmaxf(m, mt), corr = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+            l *= corr;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[d][e] *= corr;
+            m = mn;
+        }
+        const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[kb][e] = __builtin_amdgcn_exp2f(fmaf(s[kb][e], a.scale_log2, -mu));
+                l += s[kb][e];
+            }
+        if constexpr (F32) {
+#pragma unroll
+            for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float* vr = (const float*)(V + (kb * 32 + kappa(e) + 4 * h) * G::VPITCH) + fr;
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vr[32 * d], s[kb][e], o[d], 0, 0, 0);
+                }
+        } else {
+#pragma unroll
+            for (int st = 0; st < KT / 16; ++st) {
+                Vec8<T> pb;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) pb.x[j] = from_f<T>(s[st >> 1][8 * (st & 1) + j]);
+                const unsigned char* vp = V + (16 * st + tr_row) * G::VPITCH + tr_col * 2;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    const v4i16 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vp + 64 * d));
+                    const v4i16 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vp + 8 * G::VPITCH + 64 * d));
+                    const v8i16 va = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+                    o[d] = Mma32<T>::mul(*(const typename Mma<T>::frag*)&va, *(const typename Mma<T>::frag*)&pb, o[d]);
+                }
+            }
+        }
+        if (odd[t & 1] == t) {     // values set aside reach the rows that see them (whatever their weight), and no others
+            asm volatile("" ::: "memory");
+            for (int kr = 0; kr < KT; ++kr) {
+                if (!((here >> kr) & 1)) continue;
+                const int j = j0 + kr;
+                if (a.causal && j > pos) continue;
+                if (a.window && j <= pos - a.window) continue;
+                const int pi = c.by_page.div(j);
+                const T* vr = (const T*)(c.v + ((long long)c.table[b * c.table_stride + pi] * c.vs[0] +
+                                                (long long)(j - pi * c.page) * c.vs[1] + (long long)hk * c.vs[2]) * E);
+                int d0 = 4 * h;
+                asm volatile("" : "+v"(d0));       // nothing of this is kept ready for every tile
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) add_odd<T>(vr, d0 + 32 * d + kappa(i), c.dim, o[d], i);
+            }
+        }
+    };
+
+    // tile t + 1 comes into registers under tile t's products and is written to the other buffer after them; the page
+    // ids of the tile after it are on their way by then
+    if (tid < 2) odd[tid] = -1;
+    if (t0 < t1) {
+        int pg[PER];
+        pages(t0);
+        Stage s = fetch(t0);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) pg[i] = page[i];
+        pages(t0 + 1);
+        __syncthreads();
+        put(t0, s, pg);
+        __syncthreads();
+        for (int t = t0; t < t1; ++t) {
+            s = fetch(t + 1);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) pg[i] = page[i];
+            pages(t + 2);
+            if (!(a.causal && t * KT > wmax) && !idle) compute(t);
+            if (t + 1 < t1) put(t + 1, s, pg);
+            __syncthreads();
+        }
+    }
+    l = xor32_add(l);
+    if (w0 + fr >= nrows) return;
+    const int n = first + place;
+    if (a.tile_splits == 1) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        char* dst = a.o.p + ((long long)n * a.o.ts + (long long)head * a.o.hs) * E;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int dd = 32 * d + kappa(e) + 4 * h;
+                if (dd >= c.dim) continue;
+                T y[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = from_f<T>(l == 0.f ? 0.f : o[d][e + i] * inv);
+                if constexpr (F32) *(float4*)(dst + dd * E) = *(const float4*)y;
+                else *(float2*)(dst + dd * E) = *(const float2*)y;
+            }
+    } else {
+        const long long pr = (long long)split * c.tokens * a.q_heads + (long long)n * a.q_heads + head;
+        float* dst = a.part + pr * c.dim;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int dd = 32 * d + kappa(e) + 4 * h;
+                if (dd < c.dim) *(f32x4*)(dst + dd) = f32x4{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
+            }
+        if (h == 0) { a.part_ml[2 * pr] = m; a.part_ml[2 * pr + 1] = l; }
+    }
+}
+
 // Joins the splits of a row: one wave per row, the sums scaled to the splits' common maximum, then divided once.
 template <typename T>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
@@ -514,13 +860,15 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
     int first, end;
     c.rows(b, first, end);
     if (n < first) return;
+    const int splits = (end - first) * a.group <= a.rows_upto ? a.splits : a.tile_splits;
+    if (splits == 1) return;                  // written where it was computed
     float m = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[2 * (s * nrow + row)]);
+    for (int s = 0; s < splits; ++s) m = fmaxf(m, a.part_ml[2 * (s * nrow + row)]);
     const float mu = m == -INFINITY ? 0.f : m;
     float l = 0.f;
     f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
     const int d0 = lane * 4;
-    for (int s = 0; s < a.splits; ++s) {
+    for (int s = 0; s < splits; ++s) {
         const long long pr = s * nrow + row;
         const float w = __builtin_amdgcn_exp2f(a.part_ml[2 * pr] - mu);
         l += a.part_ml[2 * pr + 1] * w;
@@ -537,18 +885,31 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
 }
 
 template <typename T, int DP>
-hipError_t run_rows(const PagedAttnArgs& a, hipStream_t st) {
-    static_assert(DecGeom<T, DP>::LDS <= 150 * 1024, "LDS of a workgroup");
+hipError_t run_attention(const PagedAttnArgs& a, hipStream_t st) {
+    using R = DecGeom<T, DP>;
+    using G = TileGeom<T, DP>;
+    static_assert(R::LDS <= 150 * 1024 && G::LDS <= 150 * 1024, "LDS of a workgroup");
+    constexpr bool TILE = sizeof(T) == 2 || DP <= 128;     // as in pfm_paged_attention_plan
     const PagedKv& c = a.c;
-    // each sequence has at most one row tile that is not full
-    const long long tiles = c.cu_q ? (long long)c.tokens * a.group / 16 + c.batch
-                                   : (long long)c.batch * ((a.group + 15) / 16);
-    hipError_t e = hipFuncSetAttribute((const void*)paged_rows_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                       DecGeom<T, DP>::LDS);
-    if (e != hipSuccess) return e;
-    paged_rows_kernel<T, DP><<<dim3((unsigned)tiles, c.heads, a.splits), DEC_W * 64, DecGeom<T, DP>::LDS, st>>>(a);
-    PFM_LAUNCH_CHECK();
-    if (a.splits > 1) {
+    if (a.rows_tiles) {
+        if (R::LDS > 64 * 1024) {
+            const hipError_t e = hipFuncSetAttribute((const void*)paged_rows_kernel<T, DP>,
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, R::LDS);
+            if (e != hipSuccess) return e;
+        }
+        paged_rows_kernel<T, DP><<<dim3((unsigned)(a.rows_tiles * c.heads), a.splits), DEC_W * 64, R::LDS, st>>>(a);
+        PFM_LAUNCH_CHECK();
+    }
+    if constexpr (TILE) if (a.tiles) {
+        if (G::LDS > 64 * 1024) {
+            const hipError_t e = hipFuncSetAttribute((const void*)paged_tile_kernel<T, DP>,
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS);
+            if (e != hipSuccess) return e;
+        }
+        paged_tile_kernel<T, DP><<<dim3((unsigned)(a.tiles * c.heads), a.tile_splits), G::NW * 64, G::LDS, st>>>(a);
+        PFM_LAUNCH_CHECK();
+    }
+    if (a.splits > 1 || a.tile_splits > 1) {
         const long long rows = (long long)c.tokens * a.q_heads;
         paged_join_kernel<T><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(a);
         PFM_LAUNCH_CHECK();
@@ -557,9 +918,9 @@ hipError_t run_rows(const PagedAttnArgs& a, hipStream_t st) {
 }
 template <typename T>
 hipError_t run_attention(const PagedAttnArgs& a, hipStream_t st) {
-    if (a.c.dim <= 64) return run_rows<T, 64>(a, st);
-    if (a.c.dim <= 128) return run_rows<T, 128>(a, st);
-    return run_rows<T, 256>(a, st);
+    if (a.c.dim <= 64) return run_attention<T, 64>(a, st);
+    if (a.c.dim <= 128) return run_attention<T, 128>(a, st);
+    return run_attention<T, 256>(a, st);
 }
 
 template <typename T>
@@ -576,12 +937,33 @@ hipError_t run_append(const AppendArgs& a, hipStream_t st) {
 
 }  // namespace
 
-int pfm_paged_attention_splits(int batch, int tokens, int q_heads, int kv_heads, long long max_kv) {
-    const long long tiles = (long long)tokens * (q_heads / kv_heads) / 16 + batch;
-    const long long want = (768 + tiles * kv_heads - 1) / (tiles * kv_heads);
-    const long long most = (max_kv + KB * DEC_W - 1) / (KB * DEC_W);
-    const long long s = want < most ? want : most;
-    return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+// Which kernels run, over how many row tiles, and into how many parts each splits a sequence's keys. The sequences'
+// own lengths are on the device: sequences of at most 16 query rows (tokens x heads of a group) go to the rows kernel,
+// longer ones to the tile kernel, and both are launched where the sizes known here allow both kinds.
+void pfm_paged_attention_plan(int dtype, PagedAttnArgs& a) {
+    const PagedKv& c = a.c;
+    const long long rows = (long long)c.tokens * a.group, max_kv = (long long)c.width * c.page;
+    const int tile_rows = c.dim > 128 ? 128 : 256;
+    a.rows_upto = 16;
+    if (!c.cu_q || (dtype == DT_F32 && c.dim > 128)) {   // group rows each; or: too many registers for the tile kernel
+        a.rows_upto = 0x7fffffff;
+        a.rows_tiles = c.cu_q ? rows / 16 + c.batch : (long long)c.batch * ((a.group + 15) / 16);
+        a.tiles = 0;
+    } else {
+        a.rows_tiles = c.batch;
+        if (c.batch == 1 && rows > 16) {             // the tile kernel takes it, whatever its length is
+            a.rows_upto = 0;
+            a.rows_tiles = 0;
+        }
+        a.tiles = rows > 16 ? rows / tile_rows + std::min<long long>(c.batch, rows / 17) : 0;
+    }
+    auto parts = [&](long long units, long long fill, long long least) {
+        if (!units) return 1;
+        const long long most = (max_kv + least - 1) / least, want = (fill + units * c.heads - 1) / (units * c.heads);
+        return (int)std::max(1ll, std::min(std::min(want, most), 64ll));
+    };
+    a.splits = parts(a.rows_tiles, 768, KB * DEC_W);
+    a.tile_splits = parts(a.tiles, 256, 512);
 }
 hipError_t pfm_paged_attention(int dtype, const PagedAttnArgs& a, hipStream_t st) {
     if (dtype == DT_F32) return run_attention<float>(a, st);

@@ -76,14 +76,18 @@ struct PagedAttnArgs {
     Rows q, o;
     int q_heads, group;                 // group = q_heads / c.heads
     FastDiv by_group;
-    float scale_log2;                   // scale * log2(e)
+    float scale_log2;                   // |scale| * log2(e), or 1 for a scale of 0
+    int q_sign;                         // the scale's sign, -1, 0 or 1
     int causal, window;
-    int splits;                         // workgroups that share one row tile's keys
-    float* part;                        // splits > 1: [splits][tokens * q_heads] rows of dim sums, then max and sum
+    // the launch (pfm_paged_attention_plan)
+    int rows_upto;                      // sequences of at most so many query rows go to the rows kernel
+    long long rows_tiles, tiles;        // row tiles of the rows and of the tile kernel at most
+    int splits, tile_splits;            // workgroups that share one row tile's keys
+    float* part;                        // with splits: [splits][tokens * q_heads] rows of dim sums, then max and sum
     float* part_ml;
 };
+void pfm_paged_attention_plan(int dtype, PagedAttnArgs& a);   // of a.c, a.q_heads and a.group
 hipError_t pfm_paged_attention(int dtype, const PagedAttnArgs& a, hipStream_t st);
-int pfm_paged_attention_splits(int batch, int tokens, int q_heads, int kv_heads, long long max_kv);
 
 struct SampleArgs {
     const void* x;                      // logits [batch][ld]

@@ -2,6 +2,7 @@
 // launches. The kernels are in k_paged.hip and k_sample.hip.
 #include <math.h>
 
+#include <algorithm>
 #include <string>
 
 #include "../../include/pfm.h"
@@ -96,8 +97,9 @@ int hip(const char* fn, hipError_t e) { return e == hipSuccess ? PFM_OK : fail(f
         if (_rc) return _rc;      \
     } while (0)
 
-long long attention_ws(int splits, long long tokens, int q_heads, int dim) {
-    return splits > 1 ? splits * tokens * q_heads * (long long)(dim + 2) * 4 : 0;
+long long attention_ws(const PagedAttnArgs& a) {
+    const int s = std::max(a.splits, a.tile_splits);
+    return s > 1 ? s * (long long)a.c.tokens * a.q_heads * (a.c.dim + 2) * 4 : 0;
 }
 
 }  // namespace
@@ -141,9 +143,18 @@ int pfm_op_kv_append(void* stream, const pfm_paged_kv* cache, const pfm_rows* k,
 
 int64_t pfm_paged_attention_ws_bytes(const pfm_paged_kv* cache, int q_heads) {
     if (!cache || cache->heads < 1 || q_heads < cache->heads || cache->batch < 1 || cache->tokens < 1) return 0;
-    const int s = pfm_paged_attention_splits(cache->batch, cache->tokens, q_heads, cache->heads,
-                                             (long long)cache->table_width * cache->page_size);
-    return attention_ws(s, cache->tokens, q_heads, cache->head_dim);
+    PagedAttnArgs a{};
+    a.c.batch = cache->batch;
+    a.c.tokens = cache->tokens;
+    a.c.heads = cache->heads;
+    a.c.dim = cache->head_dim;
+    a.c.width = cache->table_width;
+    a.c.page = cache->page_size;
+    a.c.cu_q = cache->cu_q;
+    a.q_heads = q_heads;
+    a.group = q_heads / cache->heads;
+    pfm_paged_attention_plan(cache->dtype, a);
+    return attention_ws(a);
 }
 
 int pfm_op_paged_attention(void* stream, const pfm_paged_kv* cache, const pfm_rows* q, const pfm_rows* out, int q_heads,
@@ -165,17 +176,17 @@ int pfm_op_paged_attention(void* stream, const pfm_paged_kv* cache, const pfm_ro
         a.q_heads = q_heads;
         a.group = q_heads / cache->heads;
         a.by_group = fast_div((uint32_t)a.group);
-        a.scale_log2 = scale * 1.44269504088896340736f;
+        a.scale_log2 = scale == 0.f ? 1.f : fabsf(scale) * 1.44269504088896340736f;
+        a.q_sign = (scale > 0.f) - (scale < 0.f);
         a.causal = causal ? 1 : 0;
         a.window = window;
-        a.splits = pfm_paged_attention_splits(cache->batch, cache->tokens, q_heads, cache->heads,
-                                              (long long)cache->table_width * cache->page_size);
-        const long long need = attention_ws(a.splits, cache->tokens, q_heads, cache->head_dim);
+        pfm_paged_attention_plan(cache->dtype, a);
+        const long long need = attention_ws(a);
         if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
             return fail(fn, PFM_E_ARG, "workspace missing, not aligned to 16 bytes or under pfm_paged_attention_ws_bytes");
         if (need) {
             a.part = (float*)ws;
-            a.part_ml = a.part + (long long)a.splits * cache->tokens * q_heads * cache->head_dim;
+            a.part_ml = a.part + (long long)std::max(a.splits, a.tile_splits) * cache->tokens * q_heads * cache->head_dim;
         }
         const PfmDevOp ops[] = {{"q", a.q.p}, {"out", a.o.p}, {"k_pages", a.c.k}, {"v_pages", a.c.v},
                                 {"block_table", a.c.table}, {"kv_len", a.c.kv_len}, {"cu_q", a.c.cu_q},

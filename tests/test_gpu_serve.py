@@ -199,6 +199,28 @@ def test_attend_pages_and_layouts(dev, page, layout):
     attend_check(B, dev, causal=False, window=50, scale=0.3)
 
 
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-4, 1.0])
+def test_attend_scales(dev, dt, scale):
+    B = Batch([50, 1, 300], [70, 90, 310], hq=2, hk=1, D=64, dt=dt, seed=6)
+    attend_check(B, dev, scale=scale)
+    attend_check(B, dev, scale=scale, window=31)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("used,total", [(0, 40), (1, 40), (4, 300), (40, 41), (200, 300)])
+def test_attend_one_sequence_in_a_padded_call(dev, dt, used, total):
+    """One sequence whose rows fill a part of q: the rest of out stays."""
+    B = Batch([used], [used + 30], hq=4, hk=1, D=64, dt=dt, seed=used)
+    q = torch.randn(total, 4, 64).to(dt)
+    kp, vp, table, kv_len, cu = B.on(dev)
+    out = torch.full((total, 4, 64), 5.0, dtype=dt, device=dev)
+    rt.op_paged_attention(q.to(dev), kp, vp, table, kv_len, cu, out=out)
+    want, bound, spread = ref.attend(q, B.kp, B.vp, B.table, B.kv_len, B.cu, out=torch.full((total, 4, 64), 5.0))
+    assert (out[used:] == 5).all()
+    check_attend(out.cpu(), want, bound, spread, B, 64)
+
+
 def test_attend_empty_rows_and_absent_pages(dev):
     """More new tokens than keys, no keys, kv_len below 0 and above the table, pages that are not there, an idle slot."""
     B = Batch([4, 3, 2, 5, 2], [4, 3, 2, 64, 40], hq=4, hk=2, D=64, page=16, dt=BF16, width=4)
