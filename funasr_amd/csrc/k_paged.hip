@@ -6,6 +6,7 @@
 // A page id outside [0, pages) names no page: nothing is written there and its keys are not seen, so no table
 // content can reach memory outside the pages.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "pfm_serve.h"
@@ -847,34 +848,50 @@ __global__ __launch_bounds__((TileGeom<T, DP>::NW * 64), (TileGeom<T, DP>::NW / 
     }
 }
 
-// Joins the splits of a row: one wave per row, the sums scaled to the splits' common maximum, then divided once.
+// Joins the splits of one query row, one workgroup each: the splits' sums scaled to their common maximum, then divided
+// once. Rows are numbered as the kernel that split them did, `per` to a row tile.
 template <typename T>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int per, int over, int upto, int splits) {
     const PagedKv& c = a.c;
-    const int lane = threadIdx.x & 63;
-    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), nrow = (long long)c.tokens * a.q_heads;
-    if (row >= nrow) return;
-    const int n = (int)(row / a.q_heads), head = (int)(row - (long long)n * a.q_heads);
-    const int b = seq_of_row(c, n, lane);
-    if (b >= c.batch) return;                 // a row behind the last sequence: left as it is
-    int first, end;
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    const int unit = blockIdx.x / per, hk = unit % c.heads;
+    int b, tile, first, end;
+    if (!find_tile(c, a.group, per, over, upto, unit / c.heads, lane, b, tile)) return;
     c.rows(b, first, end);
-    if (n < first) return;
-    const int splits = (end - first) * a.group <= a.rows_upto ? a.splits : a.tile_splits;
-    if (splits == 1) return;                  // written where it was computed
+    const int row = tile * per + blockIdx.x % per;
+    if (row >= (end - first) * a.group) return;
+    const int place = a.by_group.div(row), n = first + place, head = hk * a.group + row - place * a.group;
+    const long long nrow = (long long)c.tokens * a.q_heads, r0 = (long long)n * a.q_heads + head;
+
     float m = -INFINITY;
-    for (int s = 0; s < splits; ++s) m = fmaxf(m, a.part_ml[2 * (s * nrow + row)]);
+    for (int s = lane; s < splits; s += 64) m = fmaxf(m, a.part_ml[2 * (s * nrow + r0)]);
+    m = wave_max(m);
     const float mu = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
+    // a lane holds 4 dims; the waves, and the parts of a wave that a row of dims does not fill, take splits in turn
+    const int lanes = c.dim <= 64 ? 16 : c.dim <= 128 ? 32 : 64, sub = lane / lanes, d0 = (lane % lanes) * 4;
+    const int step = 4 * (64 / lanes);
     f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int d0 = lane * 4;
-    for (int s = 0; s < splits; ++s) {
-        const long long pr = s * nrow + row;
+    float l = 0.f;
+#pragma unroll 4
+    for (int s = wid * (64 / lanes) + sub; s < splits; s += step) {
+        const long long pr = s * nrow + r0;
         const float w = __builtin_amdgcn_exp2f(a.part_ml[2 * pr] - mu);
         l += a.part_ml[2 * pr + 1] * w;
         if (d0 < c.dim) x += *(const f32x4*)(a.part + pr * c.dim + d0) * w;
     }
-    if (d0 >= c.dim) return;
+    for (int o = lanes; o < 64; o <<= 1) {
+        l += __shfl_xor(l, o, 64);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] += __shfl_xor(x[e], o, 64);
+    }
+    __shared__ f32x4 xs[4][64];
+    __shared__ float ls[4];
+    xs[wid][lane] = x;
+    if (lane == 0) ls[wid] = l;
+    __syncthreads();
+    if (wid || lane >= lanes || d0 >= c.dim) return;
+    l = ls[0] + ls[1] + ls[2] + ls[3];
+    x = xs[0][lane] + xs[1][lane] + xs[2][lane] + xs[3][lane];
     const float inv = l == 0.f ? 0.f : 1.f / l;
     T y[4];
 #pragma unroll
@@ -884,6 +901,26 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
     else *(float2*)dst = *(const float2*)y;
 }
 
+// More LDS than 64 KiB is asked for once per kernel and device.
+template <void (*KERNEL)(PagedAttnArgs)> hipError_t allow_lds(int bytes) {
+    static std::atomic<unsigned long long> done{0};
+    if (bytes <= 64 * 1024) return hipSuccess;
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.load() & bit)) return hipSuccess;
+    e = hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess) done.fetch_or(bit);
+    return e;
+}
+template <typename T> hipError_t run_join(const PagedAttnArgs& a, long long tiles, int per, int over, int upto, int splits,
+                                          hipStream_t st) {
+    paged_join_kernel<T><<<(unsigned)(tiles * a.c.heads * per), 256, 0, st>>>(a, per, over, upto, splits);
+    PFM_LAUNCH_CHECK();
+    return hipSuccess;
+}
+
 template <typename T, int DP>
 hipError_t run_attention(const PagedAttnArgs& a, hipStream_t st) {
     using R = DecGeom<T, DP>;
@@ -891,28 +928,22 @@ hipError_t run_attention(const PagedAttnArgs& a, hipStream_t st) {
     static_assert(R::LDS <= 150 * 1024 && G::LDS <= 150 * 1024, "LDS of a workgroup");
     constexpr bool TILE = sizeof(T) == 2 || DP <= 128;     // as in pfm_paged_attention_plan
     const PagedKv& c = a.c;
+    hipError_t e = hipSuccess;
     if (a.rows_tiles) {
-        if (R::LDS > 64 * 1024) {
-            const hipError_t e = hipFuncSetAttribute((const void*)paged_rows_kernel<T, DP>,
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, R::LDS);
-            if (e != hipSuccess) return e;
-        }
+        if ((e = allow_lds<paged_rows_kernel<T, DP>>(R::LDS)) != hipSuccess) return e;
         paged_rows_kernel<T, DP><<<dim3((unsigned)(a.rows_tiles * c.heads), a.splits), DEC_W * 64, R::LDS, st>>>(a);
         PFM_LAUNCH_CHECK();
+        const int per = c.cu_q ? 16 : std::min(16, a.group);     // a sequence's rows where they are known
+        if (a.splits > 1) e = run_join<T>(a, c.cu_q ? a.rows_tiles : (long long)c.batch * ((a.group + per - 1) / per), per,
+                                          0, a.rows_upto, a.splits, st);
+        if (e != hipSuccess) return e;
     }
     if constexpr (TILE) if (a.tiles) {
-        if (G::LDS > 64 * 1024) {
-            const hipError_t e = hipFuncSetAttribute((const void*)paged_tile_kernel<T, DP>,
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS);
-            if (e != hipSuccess) return e;
-        }
+        if ((e = allow_lds<paged_tile_kernel<T, DP>>(G::LDS)) != hipSuccess) return e;
         paged_tile_kernel<T, DP><<<dim3((unsigned)(a.tiles * c.heads), a.tile_splits), G::NW * 64, G::LDS, st>>>(a);
         PFM_LAUNCH_CHECK();
-    }
-    if (a.splits > 1 || a.tile_splits > 1) {
-        const long long rows = (long long)c.tokens * a.q_heads;
-        paged_join_kernel<T><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(a);
-        PFM_LAUNCH_CHECK();
+        if (a.tile_splits > 1) e = run_join<T>(a, a.tiles, G::ROWS, a.rows_upto, 0x7fffffff, a.tile_splits, st);
+        if (e != hipSuccess) return e;
     }
     return hipSuccess;
 }
@@ -957,13 +988,17 @@ void pfm_paged_attention_plan(int dtype, PagedAttnArgs& a) {
         }
         a.tiles = rows > 16 ? rows / tile_rows + std::min<long long>(c.batch, rows / 17) : 0;
     }
-    auto parts = [&](long long units, long long fill, long long least) {
+    // keys that one row tile sees at most: with a window its first row's reach and the rows' own span
+    auto parts = [&](long long units, long long keys, long long fill, long long least) {
         if (!units) return 1;
-        const long long most = (max_kv + least - 1) / least, want = (fill + units * c.heads - 1) / (units * c.heads);
-        return (int)std::max(1ll, std::min(std::min(want, most), 64ll));
+        const long long most = keys / least, want = (fill + units * c.heads - 1) / (units * c.heads);
+        return (int)std::max(1ll, std::min(std::min(want, most), 256ll));
     };
-    a.splits = parts(a.rows_tiles, 768, KB * DEC_W);
-    a.tile_splits = parts(a.tiles, 256, 512);
+    auto seen = [&](int rows) {
+        return a.window ? std::min<long long>(max_kv, (long long)a.window + (a.causal ? rows : c.tokens)) : max_kv;
+    };
+    a.splits = parts(a.rows_tiles, seen(16), 3072, 256);
+    a.tile_splits = parts(a.tiles, seen(tile_rows), 256, 512);
 }
 hipError_t pfm_paged_attention(int dtype, const PagedAttnArgs& a, hipStream_t st) {
     if (dtype == DT_F32) return run_attention<float>(a, st);

@@ -86,7 +86,7 @@ struct PagedAttnArgs {
     float* part;                        // with splits: [splits][tokens * q_heads] rows of dim sums, then max and sum
     float* part_ml;
 };
-void pfm_paged_attention_plan(int dtype, PagedAttnArgs& a);   // of a.c, a.q_heads and a.group
+void pfm_paged_attention_plan(int dtype, PagedAttnArgs& a);   // of a.c, a.q_heads, a.group and a.window
 hipError_t pfm_paged_attention(int dtype, const PagedAttnArgs& a, hipStream_t st);
 
 struct SampleArgs {

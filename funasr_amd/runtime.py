@@ -9,6 +9,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
+import struct
 from typing import Dict, Optional
 
 import numpy as np
@@ -76,7 +77,7 @@ class PfmVadOpts(ctypes.Structure):
 
 
 class PfmPagedKv(ctypes.Structure):
-    """pfm_paged_kv: the pages of a key / value cache, the tables and lengths of one batch."""
+    """pfm_paged_kv: the pages of a key / value cache, the tables and lengths of one batch (pass it by reference)."""
     _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_stride", ctypes.c_int64 * 3),
                 ("v_stride", ctypes.c_int64 * 3), ("pages", ctypes.c_int64), ("block_table", ctypes.c_void_p),
                 ("table_stride", ctypes.c_int64), ("kv_len", ctypes.c_void_p), ("cu_q", ctypes.c_void_p)] + \
@@ -85,7 +86,7 @@ class PfmPagedKv(ctypes.Structure):
 
 
 class PfmRows(ctypes.Structure):
-    """pfm_rows: [tokens][heads][head_dim] at any token and head stride."""
+    """pfm_rows: [tokens][heads][head_dim] at any token and head stride (pass it by reference)."""
     _fields_ = [("p", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
 
 
@@ -179,7 +180,7 @@ def load_library(path: Optional[str] = None) -> ctypes.CDLL:
     lib.pfm_vad_destroy.restype = None
     lib.pfm_streams_destroy.argtypes = [vp]
     lib.pfm_streams_destroy.restype = None
-    kvp, rows, i64 = ctypes.POINTER(PfmPagedKv), ctypes.POINTER(PfmRows), ctypes.c_int64
+    kvp, rows, i64 = vp, vp, ctypes.c_int64      # structs by reference, or their packed bytes
     lib.pfm_op_kv_append.argtypes = [vp, kvp, rows, rows, rows, rows, i32, f32p, i32, i32, i32p]
     lib.pfm_paged_attention_ws_bytes.argtypes = [kvp, i32]
     lib.pfm_paged_attention_ws_bytes.restype = i64
@@ -214,6 +215,11 @@ def _on_device(torch, device):
     if device.type != "cuda":
         raise PfmError(f"device tensors expected, got {device}")
     return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _raw_stream(torch, device) -> int:
+    """_stream_ptr without building a Stream object."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _stream_ptr(torch, device) -> int:
@@ -809,48 +815,60 @@ def op_ctc_beam(am, x, lens, ntok, beam, ctc_weight, penalty=0.0, nbest=1, sos=1
 
 
 # ---- token-by-token decoding over a paged key / value cache ---------------------------------
+# These calls are short: the descriptors are packed as the C structs' bytes, and the checks are plain comparisons.
+_KV_PACK = struct.Struct("@PPqqqqqqqPqPPiiiiiii4x").pack     # pfm_paged_kv
+_ROWS_PACK = struct.Struct("@Pqq").pack                      # pfm_rows
+
+
 def _serve_dtype(torch, t, what: str) -> int:
-    d = {torch.float32: PFM_F32, torch.bfloat16: PFM_BF16, torch.float16: PFM_F16}.get(t.dtype)
-    if d is None:
-        raise PfmError(f"{what}: float32, bfloat16 or float16 expected, got {t.dtype}")
-    return d
+    dt = t.dtype
+    if dt is torch.bfloat16:
+        return PFM_BF16
+    if dt is torch.float16:
+        return PFM_F16
+    if dt is torch.float32:
+        return PFM_F32
+    raise PfmError(f"{what}: float32, bfloat16 or float16 expected, got {dt}")
 
 
-def _vector(torch, t, n: int, dtype, device, what: str):
-    if t is not None and (t.dtype != dtype or t.shape != (n,) or t.device != device or (n > 1 and t.stride(0) != 1)):
+def _vector(t, n: int, dtype, device, what: str) -> int:
+    if t.dtype is not dtype or t.shape != (n,) or t.device != device or (n > 1 and t.stride(0) != 1):
         raise PfmError(f"{what} must be a contiguous [{n}] {dtype} tensor on {device}, got {tuple(t.shape)} {t.dtype} "
                        f"on {t.device}")
-    return t
+    return t.data_ptr()
 
 
-def _rows(t, n: int, heads: int, dim: int, dtype, device, what: str) -> PfmRows:
-    if t.shape != (n, heads, dim) or t.dtype != dtype or t.device != device:
-        raise PfmError(f"{what} must be [{n}, {heads}, {dim}] {dtype} on {device}, got {tuple(t.shape)} {t.dtype} on "
-                       f"{t.device}")
+def _rows(t, shape, dtype, device, what: str) -> bytes:
+    """pfm_rows of t, which must have this shape, type and device."""
     st = t.stride()
-    if st[2] != 1 and dim > 1:
-        raise PfmError(f"{what}: the head dimension must be contiguous")
-    return PfmRows(t.data_ptr(), st[0], st[1])
+    if t.shape != shape or t.dtype is not dtype or t.device != device or st[2] != 1:
+        raise PfmError(f"{what} must be {list(shape)} {dtype} on {device} with a contiguous head dimension, got "
+                       f"{list(t.shape)} {t.dtype} on {t.device}, strides {st}")
+    return _ROWS_PACK(t.data_ptr(), st[0], st[1])
 
 
-def _paged_kv(torch, k_pages, v_pages, block_table, kv_len, cu_q, n: int) -> PfmPagedKv:
-    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
-        raise PfmError("k_pages and v_pages must be [pages, page_size, heads, head_dim] of one shape and type")
-    dt, dev = _serve_dtype(torch, k_pages, "k_pages"), k_pages.device
-    ks, vs = k_pages.stride(), v_pages.stride()
-    if ks[3] != 1 or vs[3] != 1 or v_pages.device != dev:
-        raise PfmError("k_pages and v_pages: one device and a contiguous head dimension expected")
-    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.device != dev or \
-            (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+def _paged_kv(torch, k_pages, v_pages, block_table, kv_len, cu_q, n: int) -> bytes:
+    """pfm_paged_kv of a cache and one batch with n rows of new tokens."""
+    shape, dev = k_pages.shape, k_pages.device
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype is not k_pages.dtype or v_pages.device != dev:
+        raise PfmError("k_pages and v_pages must be [pages, page_size, heads, head_dim] of one shape, type and device")
+    dt = _serve_dtype(torch, k_pages, "k_pages")
+    P, page, heads, dim = shape
+    k0, k1, k2, k3 = k_pages.stride()
+    v0, v1, v2, v3 = v_pages.stride()
+    if k3 != 1 or v3 != 1:
+        raise PfmError("k_pages and v_pages: the head dimension must be contiguous")
+    ts = block_table.stride()
+    if len(ts) != 2 or block_table.dtype is not torch.int32 or block_table.device != dev or \
+            (ts[1] != 1 and block_table.shape[1] > 1):
         raise PfmError(f"block_table must be [batch, width] int32 on {dev} with contiguous rows")
     B, W = block_table.shape
-    _vector(torch, kv_len, B, torch.int32, dev, "kv_len")
-    _vector(torch, cu_q, B + 1, torch.int32, dev, "cu_q")
-    if cu_q is None and n != B:
+    lens = _vector(kv_len, B, torch.int32, dev, "kv_len")
+    cu = None if cu_q is None else _vector(cu_q, B + 1, torch.int32, dev, "cu_q")
+    if cu is None and n != B:
         raise PfmError(f"without cu_q every sequence has one new token: {n} rows for {B} sequences")
-    P, page, heads, dim = k_pages.shape
-    return PfmPagedKv(k_pages.data_ptr(), v_pages.data_ptr(), ks[:3], vs[:3], P, block_table.data_ptr(),
-                      block_table.stride(0) if B > 1 else W, kv_len.data_ptr(), _ptr(cu_q), dt, W, page, heads, dim, B, n)
+    return _KV_PACK(k_pages.data_ptr(), v_pages.data_ptr(), k0, k1, k2, v0, v1, v2, P, block_table.data_ptr(),
+                    ts[0] if B > 1 else W, lens, cu or 0, dt, W, page, heads, dim, B, n)
 
 
 def op_kv_append(k, v, k_pages, v_pages, block_table, kv_len, cu_q=None, q=None, inv_freq=None, interleaved=False,
@@ -861,31 +879,30 @@ def op_kv_append(k, v, k_pages, v_pages, block_table, kv_len, cu_q=None, q=None,
     sequence), pos [N] (None: the cache positions): int32; inv_freq [rot_dim / 2] f32 (None: no rotation)."""
     import torch
     lib = load_library()
-    n, dev = k.shape[0], k_pages.device
+    n, dev, dt = k.shape[0], k_pages.device, k_pages.dtype
     kv = _paged_kv(torch, k_pages, v_pages, block_table, kv_len, cu_q, n)
-    rk = _rows(k, n, kv.heads, kv.head_dim, k_pages.dtype, dev, "k")
-    rv = _rows(v, n, kv.heads, kv.head_dim, k_pages.dtype, dev, "v")
+    shape = (n, *k_pages.shape[2:])
+    rk = _rows(k, shape, dt, dev, "k")
+    rv = _rows(v, shape, dt, dev, "v")
     rq = ro = None
-    hq = 0
+    hq = rot = 0
     if q is not None:
-        if q.dim() != 3:
-            raise PfmError("q must be [tokens, q_heads, head_dim]")
         hq = q.shape[1]
-        rq = _rows(q, n, hq, kv.head_dim, k_pages.dtype, dev, "q")
+        shape = (n, hq, shape[2])
+        rq = _rows(q, shape, dt, dev, "q")
         if q_out is None:
-            q_out = torch.empty((n, hq, kv.head_dim), dtype=q.dtype, device=dev)
-        ro = _rows(q_out, n, hq, kv.head_dim, k_pages.dtype, dev, "q_out")
+            q_out = torch.empty(shape, dtype=dt, device=dev)
+        ro = _rows(q_out, shape, dt, dev, "q_out")
     elif q_out is not None:
         raise PfmError("q_out given without q")
+    freq = None
     if inv_freq is not None:
-        if inv_freq.dim() != 1:
-            raise PfmError("inv_freq must be [rot_dim / 2]")
-        _vector(torch, inv_freq, inv_freq.shape[0], torch.float32, dev, "inv_freq")
-    _vector(torch, pos, n, torch.int32, dev, "pos")
+        rot = 2 * inv_freq.shape[0]
+        freq = _vector(inv_freq, rot // 2, torch.float32, dev, "inv_freq")
+    at = None if pos is None else _vector(pos, n, torch.int32, dev, "pos")
     with _on_device(torch, dev):
-        check(lib.pfm_op_kv_append(_stream_ptr(torch, dev), kv, rk, rv, rq, ro, hq, _ptr(inv_freq),
-                                   0 if inv_freq is None else 2 * inv_freq.shape[0], 1 if interleaved else 0,
-                                   _ptr(pos)), "pfm_op_kv_append")
+        check(lib.pfm_op_kv_append(_raw_stream(torch, dev), kv, rk, rv, rq, ro, hq, freq, rot, 1 if interleaved else 0,
+                                   at), "pfm_op_kv_append")
     return q_out
 
 
@@ -898,18 +915,20 @@ def op_paged_attention(q, k_pages, v_pages, block_table, kv_len, cu_q=None, scal
     lib = load_library()
     if q.dim() != 3:
         raise PfmError("q must be [tokens, q_heads, head_dim]")
-    n, hq, dev = q.shape[0], q.shape[1], k_pages.device
+    n, hq, _ = q.shape
+    dev, dt = k_pages.device, k_pages.dtype
     kv = _paged_kv(torch, k_pages, v_pages, block_table, kv_len, cu_q, n)
-    rq = _rows(q, n, hq, kv.head_dim, k_pages.dtype, dev, "q")
+    shape = (n, hq, k_pages.shape[3])
+    rq = _rows(q, shape, dt, dev, "q")
     if out is None:
-        out = torch.empty((n, hq, kv.head_dim), dtype=q.dtype, device=dev)
-    ro = _rows(out, n, hq, kv.head_dim, k_pages.dtype, dev, "out")
+        out = torch.empty(shape, dtype=dt, device=dev)
+    ro = _rows(out, shape, dt, dev, "out")
     nb = lib.pfm_paged_attention_ws_bytes(kv, hq)
-    ws = torch.empty((nb,), dtype=torch.uint8, device=dev) if nb else None
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
     with _on_device(torch, dev):
-        check(lib.pfm_op_paged_attention(_stream_ptr(torch, dev), kv, rq, ro, hq,
-                                         kv.head_dim ** -0.5 if scale is None else float(scale), 1 if causal else 0,
-                                         int(window), _ptr(ws), nb), "pfm_op_paged_attention")
+        check(lib.pfm_op_paged_attention(_raw_stream(torch, dev), kv, rq, ro, hq,
+                                         shape[2] ** -0.5 if scale is None else scale, 1 if causal else 0, window,
+                                         ws.data_ptr() if nb else None, nb), "pfm_op_paged_attention")
     return out
 
 
@@ -919,22 +938,25 @@ def op_sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
     largest logit), top_k int32 (<= 0: off), top_p f32 (>= 1: off), min_p f32 (<= 0: off)."""
     import torch
     lib = load_library()
-    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    st = logits.stride()
+    if len(st) != 2 or (st[1] != 1 and logits.shape[1] > 1):
         raise PfmError("logits must be [B, V] with contiguous rows")
     dt, dev, (B, V) = _serve_dtype(torch, logits, "logits"), logits.device, logits.shape
     if u is None:
         raise PfmError("u, one uniform number per row, is needed")
-    for t, d, what in ((u, torch.float32, "u"), (temperature, torch.float32, "temperature"),
-                       (top_k, torch.int32, "top_k"), (top_p, torch.float32, "top_p"), (min_p, torch.float32, "min_p")):
-        _vector(torch, t, B, d, dev, what)
-    token = torch.empty((B,), dtype=torch.int32, device=dev)
-    prob = torch.empty((B,), dtype=torch.float32, device=dev)
+    f32 = torch.float32
+    settings = (_vector(u, B, f32, dev, "u"),
+                None if temperature is None else _vector(temperature, B, f32, dev, "temperature"),
+                None if top_k is None else _vector(top_k, B, torch.int32, dev, "top_k"),
+                None if top_p is None else _vector(top_p, B, f32, dev, "top_p"),
+                None if min_p is None else _vector(min_p, B, f32, dev, "min_p"))
+    token = torch.empty(B, dtype=torch.int32, device=dev)
+    prob = torch.empty(B, dtype=f32, device=dev)
     nb = lib.pfm_sample_ws_size(B, V)
-    ws = torch.empty((nb,), dtype=torch.uint8, device=dev) if nb else None
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
     with _on_device(torch, dev):
-        check(lib.pfm_op_sample(_stream_ptr(torch, dev), dt, _ptr(logits), logits.stride(0) if B > 1 else V, B, V, _ptr(u),
-                                _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(token), _ptr(prob),
-                                _ptr(ws), nb), "pfm_op_sample")
+        check(lib.pfm_op_sample(_raw_stream(torch, dev), dt, logits.data_ptr(), st[0] if B > 1 else V, B, V, *settings,
+                                token.data_ptr(), prob.data_ptr(), ws.data_ptr() if nb else None, nb), "pfm_op_sample")
     return token, prob
 
 

@@ -9,6 +9,7 @@ Tolerances (a rounding to type t is off by at most u = finfo(t).eps / 2 relative
              covers exp2 and the base change, L 2^-24 the sums over L keys; all of it relative to sum_j p_j |v_j|.
              Then u relative to the result. f16's subnormal probabilities: 2^-25 absolute per key.
   sample     the token is exact; its probability is a ratio of whole numbers rounded to f32."""
+import ctypes
 import math
 
 import numpy as np
@@ -630,9 +631,9 @@ def test_host_memory_refused(dev):
         rt.op_paged_attention(B.q, kp, vp, table, kv_len)
     with pytest.raises(rt.PfmError):
         rt.op_paged_attention(B.q.to(dev), kp, vp, B.table, kv_len)
-    lib, kv = rt.load_library(), rt._paged_kv(torch, kp, vp, table, kv_len, None, 2)
+    lib, kv = rt.load_library(), rt.PfmPagedKv.from_buffer_copy(rt._paged_kv(torch, kp, vp, table, kv_len, None, 2))
     q, host = B.q.to(dev), torch.zeros(4, dtype=torch.int32)
-    rows = rt._rows(q, 2, 4, 64, BF16, q.device, "q")
+    rows = rt._rows(q, (2, 4, 64), BF16, q.device, "q")
     kv.kv_len = host.data_ptr()
-    assert lib.pfm_op_paged_attention(None, kv, rows, rows, 4, 1.0, 1, 0, None, 0) == -1
+    assert lib.pfm_op_paged_attention(None, ctypes.byref(kv), rows, rows, 4, 1.0, 1, 0, None, 0) == -1
     assert b"kv_len" in lib.pfm_last_error()

@@ -14,6 +14,10 @@ P16 = 0x10000   # an aligned address that no check may read
 E_ARG = -1
 
 
+def ref_(x):
+    return None if x is None else ctypes.byref(x)
+
+
 def cache(**kw):
     c = rt.PfmPagedKv()
     c.k, c.v, c.pages, c.page_size, c.heads, c.head_dim, c.dtype = P16, P16, 4, 16, 2, 64, rt.PFM_BF16
@@ -24,11 +28,11 @@ def cache(**kw):
             getattr(c, k)[:] = v
         else:
             setattr(c, k, v)
-    return c
+    return ref_(c)
 
 
 def rows(p=P16, ts=256, hs=64):
-    return rt.PfmRows(p, ts, hs)
+    return ref_(rt.PfmRows(p, ts, hs))
 
 
 BAD_CACHE = [dict(dtype=2), dict(dtype=9), dict(batch=-1), dict(tokens=-1), dict(pages=-1), dict(table_width=-1),
