@@ -197,12 +197,6 @@ __device__ __forceinline__ float group_sum(float x) {
     x += __shfl_xor(x, 16, 64);
     return x + __shfl_xor(x, 32, 64);
 }
-template <typename T> __device__ __forceinline__ bool finite8(const Vec8<T>& v) {
-    bool ok = true;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ok = ok && (fabsf(to_f(v.x[i])) < INFINITY);
-    return ok;
-}
 
 // A scale's sign goes to the queries, and a scale of 0 as well (the scores' scale is 1 then): what is hidden stays at -inf.
 template <typename T> __device__ __forceinline__ T times(T x, int sign) { return from_f<T>(to_f(x) * (float)sign); }
@@ -231,12 +225,11 @@ __device__ __forceinline__ void add_odd(const T* row, int dd, int dim, V& o, int
 }
 
 constexpr int DEC_W = 4;      // waves of a workgroup; each runs over key blocks of its own
-constexpr int KB = 32;        // keys of a block
 template <typename T, int DP> struct DecGeom {
     static constexpr int PITCH = DP * sizeof(T) + (sizeof(T) == 2 ? 32 : 16);   // rows of V: no bank met twice
-    static constexpr int VB = KB * PITCH;
-    static constexpr int OFF = KB * 8;                                          // the block's V row offsets
-    static constexpr int WAVE = VB + OFF;
+    static constexpr int NT = sizeof(T) * DP > 512 ? 1 : 2;                    // 16-key tiles of a block: what registers hold
+    static constexpr int KB = 16 * NT;
+    static constexpr int WAVE = KB * PITCH;
     static constexpr int MERGE = DEC_W * 16 * (DP + 4) * 4;                     // overlays the V blocks at the end
     static constexpr int LDS = DEC_W * WAVE > MERGE ? DEC_W * WAVE : MERGE;
 };
@@ -285,7 +278,8 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
     using G = DecGeom<T, DP>;
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int ND = DP / 16;
-    constexpr int E = sizeof(T);
+    constexpr int E = sizeof(T), NT = G::NT, KB = G::KB;
+    constexpr unsigned ALL = NT == 2 ? ~0u : 0xffffu;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     __shared__ float ml[DEC_W][16][2];
     const PagedKv& c = a.c;
@@ -311,7 +305,6 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
     const int s0 = (int)((long long)nblk * split / a.splits), s1 = (int)((long long)nblk * (split + 1) / a.splits);
 
     unsigned char* Vs = smem + wid * G::WAVE;
-    long long* Vo = (long long*)(Vs + G::VB);
 
     // Q in the operand layout: 16-bit: dims 32 c + 8 g ..; 32-bit: dims 16 c + 4 g .. (the same order as K below)
     Vec8<T> qf[DP / 32];
@@ -340,93 +333,123 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
     for (int d = 0; d < ND; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
 
-    for (int blk = s0 + wid; blk < s1; blk += DEC_W) {
+    // The lane's key rows of a block are j0 + r and j0 + 16 + r, of K (operand layout as it is) and of V alike. A block is
+    // loaded while the one before it is worked on: its K goes into the registers that the products have just read, its
+    // V into those that LDS has just taken, and the page ids of the block after it are on their way.
+    constexpr int NL = DP * E / 64;              // 16-byte pieces of a row that a lane holds: at 64 k + 16 g
+    float4 kf[NT][NL], vf[NT][NL];
+    int page[NT];                                // of the block to be loaded next; -1: no such key
+    long long ko[NT], vo[NT];
+    unsigned here = 0;                           // keys of the loaded block that exist
+    auto pages = [&](int blk) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int j = (blk0 + blk) * KB + 16 * t + r;
+            page[t] = -1;
+            if (blk < s1 && j >= lo && j < hi) page[t] = c.table[b * c.table_stride + c.by_page.div(j)];
+            if ((unsigned long long)(long long)page[t] >= (unsigned long long)c.pages) page[t] = -1;
+        }
+    };
+    auto address = [&](int blk) {
+        here = (unsigned)(__ballot(page[0] >= 0) & 0xffff);
+        if constexpr (NT == 2) here |= (unsigned)(__ballot(page[NT - 1] >= 0) & 0xffff) << 16;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int j = (blk0 + blk) * KB + 16 * t + r, slot = j - c.by_page.div(j) * c.page;
+            ko[t] = ((long long)page[t] * c.ks[0] + (long long)slot * c.ks[1] + (long long)hk * c.ks[2]) * E + 16 * g;
+            vo[t] = ((long long)page[t] * c.vs[0] + (long long)slot * c.vs[1] + (long long)hk * c.vs[2]) * E + 16 * g;
+        }
+        if (here != ALL && here) {               // rows that are not there read one that is
+            const int f = __ffs((int)here) - 1;
+            const long long k1 = __shfl(f < 16 ? ko[0] : ko[NT - 1], (f & 15) + 16 * g, 64);
+            const long long v1 = __shfl(f < 16 ? vo[0] : vo[NT - 1], (f & 15) + 16 * g, 64);
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+                if (page[t] < 0) { ko[t] = k1; vo[t] = v1; }
+        }
+    };
+    // pieces behind the head's dims read its last ones: their K is cleared, their V is not used
+    auto load = [&](const char* base, const long long (&off)[NT], float4 (&x)[NT][NL]) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int k = 0; k < NL; ++k)
+                x[t][k] = *(const float4*)(base + off[t] + min(64 * k, c.dim * E - 16 - 16 * g));
+    };
+    int blk = s0 + wid;
+    pages(blk);
+    address(blk);
+    if (here) { load(c.k, ko, kf); load(c.v, vo, vf); }
+    pages(blk + DEC_W);
+
+    for (; blk < s1; blk += DEC_W) {
         const int j0 = (blk0 + blk) * KB;
-        // the lane's key rows j0 + r and j0 + 16 + r; -1: no such key
-        long long ko[2];
-        bool here[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int j = j0 + 16 * t + r;
-            here[t] = j >= lo && j < hi;
-            long long vo = -1;
-            ko[t] = 0;
-            if (here[t]) {
-                const int pi = c.by_page.div(j), slot = j - pi * c.page;
-                const long long pg = page_of(c, b, pi);
-                here[t] = pg >= 0;
-                if (here[t]) {
-                    ko[t] = (pg * c.ks[0] + (long long)slot * c.ks[1] + (long long)hk * c.ks[2]) * E;
-                    vo = (pg * c.vs[0] + (long long)slot * c.vs[1] + (long long)hk * c.vs[2]) * E;
-                }
-            }
-            if (g == 0) Vo[16 * t + r] = vo;
-        }
-        __builtin_amdgcn_wave_barrier();
+        const unsigned there = here;
         // keys this lane's scores belong to (rows 4 g + i of each tile) that exist
-        unsigned exist;
-        {
-            const unsigned e0 = (unsigned)(__ballot(here[0]) & 0xffff), e1 = (unsigned)(__ballot(here[1]) & 0xffff);
-            exist = ((e0 >> (4 * g)) & 15) | (((e1 >> (4 * g)) & 15) << 4);
-        }
+        const unsigned exist = ((there >> (4 * g)) & 15) | ((there >> (16 + 4 * g)) & 15) << 4;
         // S^T = K Q^T
-        f32x4 s[2];
+        f32x4 s[NT];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < NT; ++t) {
             s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-            Vec8<T> kf[DP / 32];
 #pragma unroll
-            for (int k = 0; k < DP / 32; ++k) {
-                const int d0 = F32 ? 32 * k + 4 * g : 32 * k + 8 * g;
-                kf[k] = Vec8<T>{};
+            for (int k = 0; k < NL; ++k) {
+                float4 x = kf[t][k];
+                if (DP * E > c.dim * E && 64 * k + 16 * g >= c.dim * E) x = make_float4(0.f, 0.f, 0.f, 0.f);
                 if constexpr (F32) {
-                    if (here[t] && d0 < c.dim) ((float4*)&kf[k])[0] = *(const float4*)(c.k + ko[t] + d0 * E);
-                    if (here[t] && d0 + 16 < c.dim) ((float4*)&kf[k])[1] = *(const float4*)(c.k + ko[t] + (d0 + 16) * E);
-                } else if (here[t] && d0 < c.dim) {
-                    kf[k] = load8<T>(c.k + ko[t] + d0 * E);
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < DP / 32; ++k) {
-                if constexpr (F32) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[k].x[e], qf[k].x[e], s[t], 0, 0, 0);
+                    const float4 q4 = ((const float4*)qf)[k];
+                    s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.x, q4.x, s[t], 0, 0, 0);
+                    s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.y, q4.y, s[t], 0, 0, 0);
+                    s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.z, q4.z, s[t], 0, 0, 0);
+                    s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.w, q4.w, s[t], 0, 0, 0);
                 } else {
-                    s[t] = Mma<T>::mul(*(typename Mma<T>::frag*)&kf[k], *(typename Mma<T>::frag*)&qf[k], s[t]);
+                    s[t] = Mma<T>::mul(*(typename Mma<T>::frag*)&x, *(typename Mma<T>::frag*)&qf[k], s[t]);
                 }
             }
         }
+        address(blk + DEC_W);
+        if (here) load(c.k, ko, kf);
         // V rows into LDS, absent ones as zeros
-        const bool edge = j0 < lo || j0 + KB > hi || (a.causal && j0 + KB - 1 > pmin) || (a.window && j0 <= pmax - a.window);
-        bool odd = false;     // a value that is not finite, in a block that some row sees in part
-        constexpr int CPR = DP / 8;      // 8-wide pieces of a row
+        // (rows at one position see the same keys, and the others are not there)
+        const bool part = pmin < pmax && ((a.causal && j0 + KB - 1 > pmin) || (a.window && j0 <= pmax - a.window));
+        bool odd = false;     // a value that is not finite, in a block that the rows do not all see whole
+        if (there != ALL) {
+            asm volatile("" ::: "memory");       // branches of their own: not folded into every block
 #pragma unroll
-        for (int i = 0; i < KB * CPR / 64; ++i) {
-            const int q8 = i * 64 + lane, kr = q8 / CPR, d0 = (q8 % CPR) * 8;
-            const long long vo = Vo[kr];
-            Vec8<T> v = Vec8<T>{};
-            if (vo >= 0 && d0 < c.dim) v = load8<T>(c.v + vo + d0 * E);
-            if (edge && !finite8(v)) {
-                odd = true;
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (!(fabsf(to_f(v.x[e])) < INFINITY)) v.x[e] = from_f<T>(0.f);
-            }
-            store8<T>((char*)Vs + kr * G::PITCH + d0 * E, v);
+                for (int k = 0; k < NL; ++k)
+                    if (!((there >> (16 * t + r)) & 1)) vf[t][k] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
+        if (part) {
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int k = 0; k < NL; ++k) {
+                    const float4 x = vf[t][k];
+                    vf[t][k] = make_float4(finite_word<T>(x.x, odd), finite_word<T>(x.y, odd), finite_word<T>(x.z, odd),
+                                           finite_word<T>(x.w, odd));
+                }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int k = 0; k < NL; ++k) *(float4*)(Vs + (16 * t + r) * G::PITCH + 64 * k + 16 * g) = vf[t][k];
+        if (here) load(c.v, vo, vf);
+        pages(blk + 2 * DEC_W);
         // scores in base-2 exponents; a key that the row does not see is replaced, whatever its score is
         unsigned seen = exist;
-        if (edge) {
+        if (part) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
+            for (int e = 0; e < 4 * NT; ++e) {
                 const int j = j0 + 16 * (e >> 2) + 4 * g + (e & 3);
                 if ((a.causal && j > pos) || (a.window && j <= pos - a.window)) seen &= ~(1u << e);
             }
         }
         float mt = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < 4 * NT; ++e) {
             float x = s[e >> 2][e & 3] * a.scale_log2;
             x = (seen >> e) & 1 ? x : -INFINITY;
             s[e >> 2][e & 3] = x;
@@ -436,9 +459,9 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
         const float mn = fmaxf(m, mt), mu = mn == -INFINITY ? 0.f : mn;
         const float corr = __builtin_amdgcn_exp2f(m - mu);
         m = mn;
-        float p[8], ls = 0.f;
+        float p[4 * NT], ls = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < 4 * NT; ++e) {
             p[e] = __builtin_amdgcn_exp2f(s[e >> 2][e & 3] - mu);
             ls += p[e];
         }
@@ -449,7 +472,7 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
         __builtin_amdgcn_wave_barrier();
         if constexpr (F32) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
+            for (int e = 0; e < 4 * NT; ++e) {
                 const float* vr = (const float*)(Vs + (16 * (e >> 2) + 4 * g + (e & 3)) * G::PITCH) + r;
 #pragma unroll
                 for (int d = 0; d < ND; ++d) o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[16 * d], p[e], o[d], 0, 0, 0);
@@ -470,16 +493,17 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
         }
         // values that are not finite belong to the rows that see them only (whatever their weight): 0 x inf in the product
         // would reach the rest
-        if (edge && __any(odd)) {
+        if (part && __any(odd)) {
             for (int kr = 0; kr < KB; ++kr) {
-                const long long vo = Vo[kr];
-                if (vo < 0) continue;
                 const int j = j0 + kr;
-                if ((a.causal && j > pos) || (a.window && j <= pos - a.window)) continue;
+                if (!((there >> kr) & 1) || (a.causal && j > pos) || (a.window && j <= pos - a.window)) continue;
+                const int pi = c.by_page.div(j);
+                const T* vr = (const T*)(c.v + (page_of(c, b, pi) * c.vs[0] + (long long)(j - pi * c.page) * c.vs[1] +
+                                                (long long)hk * c.vs[2]) * E);
                 int d0 = 4 * g;
                 asm volatile("" : "+v"(d0));       // nothing of this is kept ready for every block
 #pragma unroll
-                for (int d = 0; d < ND; ++d) add_odd<T>((const T*)(c.v + vo), d0 + 16 * d, c.dim, o[d], 0);
+                for (int d = 0; d < ND; ++d) add_odd<T>(vr, d0 + 16 * d, c.dim, o[d], 0);
             }
         }
         __builtin_amdgcn_wave_barrier();
@@ -863,34 +887,36 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int pe
     const int place = a.by_group.div(row), n = first + place, head = hk * a.group + row - place * a.group;
     const long long nrow = (long long)c.tokens * a.q_heads, r0 = (long long)n * a.q_heads + head;
 
-    float m = -INFINITY;
-    for (int s = lane; s < splits; s += 64) m = fmaxf(m, a.part_ml[2 * (s * nrow + r0)]);
-    m = wave_max(m);
-    const float mu = m == -INFINITY ? 0.f : m;
+    // the splits' weights (at most one per thread)
+    __shared__ float ws[256], ms[4], ls[4];
+    __shared__ f32x4 xs[4][64];
+    const int t = threadIdx.x;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (t < splits) ml = *(const float2*)(a.part_ml + 2 * (t * nrow + r0));
+    const float mw = wave_max(ml.x);
+    if (lane == 0) ms[wid] = mw;
+    __syncthreads();
+    const float m = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]));
+    const float w = __builtin_amdgcn_exp2f(ml.x - (m == -INFINITY ? 0.f : m));
+    ws[t] = w;
+    const float lw = wave_sum(ml.y * w);
+    if (lane == 0) ls[wid] = lw;
+    __syncthreads();
     // a lane holds 4 dims; the waves, and the parts of a wave that a row of dims does not fill, take splits in turn
     const int lanes = c.dim <= 64 ? 16 : c.dim <= 128 ? 32 : 64, sub = lane / lanes, d0 = (lane % lanes) * 4;
     const int step = 4 * (64 / lanes);
     f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
-#pragma unroll 4
-    for (int s = wid * (64 / lanes) + sub; s < splits; s += step) {
-        const long long pr = s * nrow + r0;
-        const float w = __builtin_amdgcn_exp2f(a.part_ml[2 * pr] - mu);
-        l += a.part_ml[2 * pr + 1] * w;
-        if (d0 < c.dim) x += *(const f32x4*)(a.part + pr * c.dim + d0) * w;
-    }
+#pragma unroll 8
+    for (int s = wid * (64 / lanes) + sub; s < splits; s += step)
+        if (d0 < c.dim) x += *(const f32x4*)(a.part + (s * nrow + r0) * c.dim + d0) * ws[s];
     for (int o = lanes; o < 64; o <<= 1) {
-        l += __shfl_xor(l, o, 64);
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] += __shfl_xor(x[e], o, 64);
     }
-    __shared__ f32x4 xs[4][64];
-    __shared__ float ls[4];
     xs[wid][lane] = x;
-    if (lane == 0) ls[wid] = l;
     __syncthreads();
     if (wid || lane >= lanes || d0 >= c.dim) return;
-    l = ls[0] + ls[1] + ls[2] + ls[3];
+    const float l = ls[0] + ls[1] + ls[2] + ls[3];
     x = xs[0][lane] + xs[1][lane] + xs[2][lane] + xs[3][lane];
     const float inv = l == 0.f ? 0.f : 1.f / l;
     T y[4];
@@ -995,9 +1021,9 @@ void pfm_paged_attention_plan(int dtype, PagedAttnArgs& a) {
         return (int)std::max(1ll, std::min(std::min(want, most), 256ll));
     };
     auto seen = [&](int rows) {
-        return a.window ? std::min<long long>(max_kv, (long long)a.window + (a.causal ? rows : c.tokens)) : max_kv;
+        return a.window ? std::min<long long>(max_kv, (long long)a.window + rows + (a.causal ? 0 : rows == 16 ? std::min(a.rows_upto, c.tokens) : c.tokens)) : max_kv;
     };
-    a.splits = parts(a.rows_tiles, seen(16), 3072, 256);
+    a.splits = parts(a.rows_tiles, seen(16), 2048, 256);
     a.tile_splits = parts(a.tiles, seen(tile_rows), 256, 512);
 }
 hipError_t pfm_paged_attention(int dtype, const PagedAttnArgs& a, hipStream_t st) {
