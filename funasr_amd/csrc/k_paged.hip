@@ -6,7 +6,6 @@
 // A page id outside [0, pages) names no page: nothing is written there and its keys are not seen, so no table
 // content can reach memory outside the pages.
 #include <algorithm>
-#include <atomic>
 #include <type_traits>
 
 #include "pfm_serve.h"
@@ -927,19 +926,6 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int pe
     else *(float2*)dst = *(const float2*)y;
 }
 
-// More LDS than 64 KiB is asked for once per kernel and device.
-template <void (*KERNEL)(PagedAttnArgs)> hipError_t allow_lds(int bytes) {
-    static std::atomic<unsigned long long> done{0};
-    if (bytes <= 64 * 1024) return hipSuccess;
-    int dev = 0;
-    hipError_t e = hipGetDevice(&dev);
-    if (e != hipSuccess) return e;
-    const unsigned long long bit = 1ull << (dev & 63);
-    if (dev < 64 && (done.load() & bit)) return hipSuccess;
-    e = hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == hipSuccess) done.fetch_or(bit);
-    return e;
-}
 template <typename T> hipError_t run_join(const PagedAttnArgs& a, long long tiles, int per, int over, int upto, int splits,
                                           hipStream_t st) {
     paged_join_kernel<T><<<(unsigned)(tiles * a.c.heads * per), 256, 0, st>>>(a, per, over, upto, splits);
@@ -956,7 +942,7 @@ hipError_t run_attention(const PagedAttnArgs& a, hipStream_t st) {
     const PagedKv& c = a.c;
     hipError_t e = hipSuccess;
     if (a.rows_tiles) {
-        if ((e = allow_lds<paged_rows_kernel<T, DP>>(R::LDS)) != hipSuccess) return e;
+        if ((e = pfm_allow_lds<paged_rows_kernel<T, DP>>(R::LDS)) != hipSuccess) return e;
         paged_rows_kernel<T, DP><<<dim3((unsigned)(a.rows_tiles * c.heads), a.splits), DEC_W * 64, R::LDS, st>>>(a);
         PFM_LAUNCH_CHECK();
         const int per = c.cu_q ? 16 : std::min(16, a.group);     // a sequence's rows where they are known
@@ -965,7 +951,7 @@ hipError_t run_attention(const PagedAttnArgs& a, hipStream_t st) {
         if (e != hipSuccess) return e;
     }
     if constexpr (TILE) if (a.tiles) {
-        if ((e = allow_lds<paged_tile_kernel<T, DP>>(G::LDS)) != hipSuccess) return e;
+        if ((e = pfm_allow_lds<paged_tile_kernel<T, DP>>(G::LDS)) != hipSuccess) return e;
         paged_tile_kernel<T, DP><<<dim3((unsigned)(a.tiles * c.heads), a.tile_splits), G::NW * 64, G::LDS, st>>>(a);
         PFM_LAUNCH_CHECK();
         if (a.tile_splits > 1) e = run_join<T>(a, a.tiles, G::ROWS, a.rows_upto, 0x7fffffff, a.tile_splits, st);

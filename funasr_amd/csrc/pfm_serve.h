@@ -1,6 +1,8 @@
 // Token-by-token decoding over a paged key / value cache: argument blocks shared by the kernels (k_paged.hip,
 // k_sample.hip) and their C entry points (pfm_serve.hip).
 #pragma once
+#include <atomic>
+
 #include "pfm_common.h"
 
 typedef _Float16 f16;
@@ -30,6 +32,19 @@ static inline FastDiv fast_div(uint32_t d) {
     return f;
 }
 
+// More LDS than 64 KiB is asked for once per kernel and device.
+template <auto KERNEL> hipError_t pfm_allow_lds(int bytes) {
+    static std::atomic<unsigned long long> done{0};
+    if (bytes <= 64 * 1024) return hipSuccess;
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.load() & bit)) return hipSuccess;
+    e = hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess) done.fetch_or(bit);
+    return e;
+}
 // A batch of sequences whose keys and values lie in pages. Strides count elements; the head dimension is contiguous.
 struct PagedKv {
     char *k, *v;                        // pages
