@@ -26,7 +26,7 @@ __device__ __forceinline__ int seq_of_row(const PagedKv& c, int n, int lane) {
     return b;
 }
 
-__device__ __forceinline__ long long page_of(const PagedKv& c, int b, int t) {   // t inside the table's reach
+__device__ __forceinline__ int page_of(const PagedKv& c, int b, int t) {   // t inside the table's reach
     const int pg = c.table[b * c.table_stride + t];
     return pg >= 0 && pg < c.pages ? pg : -1;
 }
@@ -52,7 +52,7 @@ constexpr int AP_T = 256;
 template <typename T, int TB>
 __global__ __launch_bounds__(AP_T) void kv_append_kernel(AppendArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    __shared__ long long dst_page[TB];
+    __shared__ int dst_page[TB];
     __shared__ int dst_slot[TB];            // -1: the row has no sequence; -2: rotated, but no place to write
     __shared__ int turn_pos[TB];
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
@@ -64,7 +64,7 @@ __global__ __launch_bounds__(AP_T) void kv_append_kernel(AppendArgs a) {
     for (int t = wid; t < TB; t += AP_T / 64) {
         const int n = n0 + t;
         int slot = -1, pos = 0;
-        long long page = 0;
+        int page = 0;
         if (n < c.tokens) {
             const int b = seq_of_row(c, n, lane);
             int first, end;
@@ -123,7 +123,7 @@ __global__ __launch_bounds__(AP_T) void kv_append_kernel(AppendArgs a) {
                 h -= a.q_heads;
                 if (slot < 0) continue;
                 src = a.k.p + ((long long)n * a.k.ts + (long long)h * a.k.hs) * E;
-                dst = c.k + (dst_page[t] * c.ks[0] + (long long)slot * c.ks[1] + (long long)h * c.ks[2]) * E;
+                dst = c.k_head(h) + c.k_at(dst_page[t], slot);
             }
             if (!turn) {
                 const int o = (2 * h8 + j) * 8 * E;
@@ -159,7 +159,7 @@ __global__ __launch_bounds__(AP_T) void kv_append_kernel(AppendArgs a) {
             w -= turned + kept;
             if (slot < 0) continue;
             const int h = w / D8, o = (w - h * D8) * 8 * E;
-            store8<T>(c.v + (dst_page[t] * c.vs[0] + (long long)slot * c.vs[1] + (long long)h * c.vs[2]) * E + o,
+            store8<T>(c.v_head(h) + c.v_at(dst_page[t], slot) + o,
                       load8<T>(a.v.p + ((long long)n * a.v.ts + (long long)h * a.v.hs) * E + o));
         }
     }
@@ -223,6 +223,9 @@ __device__ __forceinline__ void add_odd(const T* row, int dd, int dim, V& o, int
     }
 }
 
+// a value that is the same in all lanes, as a scalar
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 constexpr int DEC_W = 4;      // waves of a workgroup; each runs over key blocks of its own
 template <typename T, int DP> struct DecGeom {
     static constexpr int PITCH = DP * sizeof(T) + (sizeof(T) == 2 ? 32 : 16);   // rows of V: no bank met twice
@@ -262,10 +265,10 @@ __device__ __forceinline__ bool find_tile(const PagedKv& c, int group, int rows,
         if (past) {
             const int l = __ffsll((long long)past) - 1;
             b = i0 + l;
-            tile = x - __shfl(sum - tiles, l, 64);
+            tile = x - __builtin_amdgcn_readlane(sum - tiles, l);
             return true;
         }
-        x -= __shfl(sum, 63, 64);
+        x -= __builtin_amdgcn_readlane(sum, 63);
     }
     return false;
 }
@@ -282,14 +285,17 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     __shared__ float ml[DEC_W][16][2];
     const PagedKv& c = a.c;
-    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wid = uniform(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
     const int hk = blockIdx.x % c.heads;
     int b, tile;
     if (!find_tile(c, a.group, 16, 0, a.rows_upto, blockIdx.x / c.heads, lane, b, tile)) return;
+    b = uniform(b);
+    tile = uniform(tile);
     int first, end;
     c.rows(b, first, end);
-    const int nq = end - first, len = c.len(b);
+    first = uniform(first);
+    const int nq = uniform(end) - first, len = uniform(c.len(b));
     const int rows = min(16, nq * a.group - tile * 16);            // of this tile
     const int row = min(tile * 16 + r, nq * a.group - 1);
     const int place = a.by_group.div(row);
@@ -355,13 +361,13 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const int j = (blk0 + blk) * KB + 16 * t + r, slot = j - c.by_page.div(j) * c.page;
-            ko[t] = ((long long)page[t] * c.ks[0] + (long long)slot * c.ks[1] + (long long)hk * c.ks[2]) * E + 16 * g;
-            vo[t] = ((long long)page[t] * c.vs[0] + (long long)slot * c.vs[1] + (long long)hk * c.vs[2]) * E + 16 * g;
+            ko[t] = (long long)c.k_at(page[t], slot);
+            vo[t] = (long long)c.v_at(page[t], slot);
         }
         if (here != ALL && here) {               // rows that are not there read one that is
             const int f = __ffs((int)here) - 1;
-            const long long k1 = __shfl(f < 16 ? ko[0] : ko[NT - 1], (f & 15) + 16 * g, 64);
-            const long long v1 = __shfl(f < 16 ? vo[0] : vo[NT - 1], (f & 15) + 16 * g, 64);
+            const long long k1 = __shfl(f < 16 ? ko[0] : ko[NT - 1], f & 15, 64);
+            const long long v1 = __shfl(f < 16 ? vo[0] : vo[NT - 1], f & 15, 64);
 #pragma unroll
             for (int t = 0; t < NT; ++t)
                 if (page[t] < 0) { ko[t] = k1; vo[t] = v1; }
@@ -375,10 +381,11 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
             for (int k = 0; k < NL; ++k)
                 x[t][k] = *(const float4*)(base + off[t] + min(64 * k, c.dim * E - 16 - 16 * g));
     };
+    const char *k0 = c.k_head(hk) + 16 * g, *v0 = c.v_head(hk) + 16 * g;
     int blk = s0 + wid;
     pages(blk);
     address(blk);
-    if (here) { load(c.k, ko, kf); load(c.v, vo, vf); }
+    if (here) { load(k0, ko, kf); load(v0, vo, vf); }
     pages(blk + DEC_W);
 
     for (; blk < s1; blk += DEC_W) {
@@ -407,7 +414,7 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
             }
         }
         address(blk + DEC_W);
-        if (here) load(c.k, ko, kf);
+        if (here) load(k0, ko, kf);
         // V rows into LDS, absent ones as zeros
         // (rows at one position see the same keys, and the others are not there)
         const bool part = pmin < pmax && ((a.causal && j0 + KB - 1 > pmin) || (a.window && j0 <= pmax - a.window));
@@ -435,7 +442,7 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int k = 0; k < NL; ++k) *(float4*)(Vs + (16 * t + r) * G::PITCH + 64 * k + 16 * g) = vf[t][k];
-        if (here) load(c.v, vo, vf);
+        if (here) load(v0, vo, vf);
         pages(blk + 2 * DEC_W);
         // scores in base-2 exponents; a key that the row does not see is replaced, whatever its score is
         unsigned seen = exist;
@@ -497,8 +504,7 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
                 const int j = j0 + kr;
                 if (!((there >> kr) & 1) || (a.causal && j > pos) || (a.window && j <= pos - a.window)) continue;
                 const int pi = c.by_page.div(j);
-                const T* vr = (const T*)(c.v + (page_of(c, b, pi) * c.vs[0] + (long long)(j - pi * c.page) * c.vs[1] +
-                                                (long long)hk * c.vs[2]) * E);
+                const T* vr = (const T*)(c.v_head(hk) + c.v_at(page_of(c, b, pi), j - pi * c.page));
                 int d0 = 4 * g;
                 asm volatile("" : "+v"(d0));       // nothing of this is kept ready for every block
 #pragma unroll
@@ -581,21 +587,26 @@ template <> struct Mma32<f16> {
     }
 };
 
+typedef __attribute__((address_space(3))) void lds_void;
+typedef const __attribute__((address_space(1))) void gbl_void;
+
 template <typename T, int DP> struct TileGeom {
     static constexpr int E = sizeof(T);
     static constexpr int NW = DP > 128 ? 4 : 8;            // waves: 256 registers each suffice up to 128 dims
     static constexpr int ROWS = NW * 32;
     static constexpr int KT = E == 2 && DP <= 128 ? 64 : 32;   // keys of a tile
-    static constexpr int CPR = DP * E / 16;                // 16-byte pieces of a row
-    static constexpr int KPITCH = E == 2 ? DP * 2 : DP * 4 + 16;
-    static constexpr int VPITCH = E == 2 ? DP * 2 + 64 : DP * 4;
-    static constexpr int STAGE = KT * (KPITCH + VPITCH);
-    static constexpr int LDS = 2 * STAGE;
+    static constexpr int PITCH = DP * E;                   // a row of K or V
+    static constexpr int CPR = PITCH / 16;                 // its 16-byte pieces
+    static constexpr int TILE = KT * PITCH;
+    static constexpr int RING = 4;                         // tiles of K, and of V, in LDS
+    static constexpr int LDS = 2 * RING * TILE;
     static constexpr int PER = KT * CPR / (NW * 64);       // pieces of K, and of V, that a thread brings
-    // place of piece c of key row r: the 16 rows that a read of one piece column touches lie in different banks
-    static __device__ __forceinline__ int kpiece(int r, int c) {
-        if (E == 4) return c;
-        return CPR == 8 ? c ^ ((r >> 1) & 7) : c ^ (r & 15);
+    // Piece c of row r lies at place c ^ swizzle(r), so that a read meets each bank as often as it must: of K, one piece
+    // column of 16 rows; of V, four pieces of 8 rows (transposing reads) or 8 pieces of the rows r and r + 4.
+    static __device__ __forceinline__ int kswizzle(int r) { return CPR == 8 ? (r >> 1) & 7 : r & 15; }
+    static __device__ __forceinline__ int vswizzle(int r) {
+        if (E == 4) return ((r >> 2) & 1) << 3;
+        return CPR == 8 ? ((r >> 1) & 1) << 2 : ((r & 3) << 2) | ((r >> 2) & 3);
     }
 };
 
@@ -606,16 +617,19 @@ __global__ __launch_bounds__((TileGeom<T, DP>::NW * 64), (TileGeom<T, DP>::NW / 
     constexpr int E = sizeof(T), KT = G::KT, NB = KT / 32, ND = DP / 32, NT = G::NW * 64;
     constexpr int NQ = DP * E / 32;                          // 16-byte pieces of a query row that a lane holds
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    __shared__ unsigned char there[2][KT];                   // the tile's keys that exist
+    __shared__ unsigned char there[G::RING][KT];                 // a tile's keys that exist
     __shared__ int odd[2];                                   // the last tile of a buffer with a value that is not finite
     const PagedKv& c = a.c;
-    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, fr = lane & 31, h = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wid = uniform(tid >> 6), fr = lane & 31, h = lane >> 5;
     const int hk = blockIdx.x % c.heads;
     int b, tile;
     if (!find_tile(c, a.group, G::ROWS, a.rows_upto, 0x7fffffff, (gridDim.x - 1 - blockIdx.x) / c.heads, lane, b, tile)) return;
+    b = uniform(b);
+    tile = uniform(tile);
     int first, end;
     c.rows(b, first, end);
-    const int nq = end - first, len = c.len(b), nrows = nq * a.group, base = len - nq;
+    first = uniform(first);
+    const int nq = uniform(end) - first, len = uniform(c.len(b)), nrows = nq * a.group, base = len - nq;
     const int row0 = tile * G::ROWS, row1 = min(row0 + G::ROWS, nrows) - 1;
     const int pmin = base + a.by_group.div(row0), pmax = base + a.by_group.div(row1);
     // this wave's rows; -1 rows: none
@@ -654,70 +668,91 @@ __global__ __launch_bounds__((TileGeom<T, DP>::NW * 64), (TileGeom<T, DP>::NW / 
         for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
     float m = -INFINITY, l = 0.f;
 
-    // staging: the thread's pieces are column tid % CPR of the rows tid / CPR + i NT / CPR
-    constexpr int PER = G::PER, RSTEP = NT / G::CPR;
+    // Staging: global memory straight to LDS, 1 KiB per instruction of a wave: its pieces lie side by side there, so the
+    // lane picks the piece that belongs to its place. The thread's places are piece tid % CPR of the rows tid / CPR +
+    // i NT / CPR; what is not there is not loaded, and its V is cleared.
+    constexpr int PER = G::PER, RSTEP = NT / G::CPR, RING = G::RING;
+    unsigned char *K0 = smem, *V0 = smem + RING * G::TILE;
     const int scol = tid % G::CPR, srow = tid / G::CPR;
-    const bool in_dim = scol * 16 < c.dim * E;
-    int page[PER];
-    auto pages = [&](int t) {          // page ids of tile t's rows; -1: no such key
+    int page[PER];                       // page ids of the tile that comes next; -1: no such key
+    auto pages = [&](int t) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int j = t * KT + srow + i * RSTEP;
-            page[i] = -1;
-            if (j >= lo && j < hi) page[i] = c.table[b * c.table_stride + c.by_page.div(j)];
-            if ((unsigned long long)(long long)page[i] >= (unsigned long long)c.pages) page[i] = -1;
+            const int j = t * KT + srow + i * RSTEP, at = min(max(j, lo), hi - 1);
+            page[i] = c.table[b * c.table_stride + c.by_page.div(at)];
+            if (at != j) page[i] = -1;
         }
     };
-    struct Stage { float4 k[PER], v[PER]; };
-    const char* kb0 = c.k + ((long long)hk * c.ks[2]) * E + scol * 16;
-    const char* vb0 = c.v + ((long long)hk * c.vs[2]) * E + scol * 16;
-    auto fetch = [&](int t) -> Stage {
-        Stage s;
+    bool full = false;                   // this wave made 2 PER loads for the last tile brought
+    auto bring = [&](int t) {
+        unsigned char *K = K0 + (t % RING) * G::TILE + wid * 1024, *V = V0 + (t % RING) * G::TILE + wid * 1024;
+        full = true;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int j = t * KT + srow + i * RSTEP, slot = j - c.by_page.div(j) * c.page;
-            s.k[i] = s.v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (page[i] >= 0 && in_dim) {
-                s.k[i] = *(const float4*)(kb0 + ((long long)page[i] * c.ks[0] + (long long)slot * c.ks[1]) * E);
-                s.v[i] = *(const float4*)(vb0 + ((long long)page[i] * c.vs[0] + (long long)slot * c.vs[1]) * E);
-            }
+            const int r = srow + i * RSTEP, j = t * KT + r, slot = j - c.by_page.div(j) * c.page;
+            const int kc = scol ^ G::kswizzle(r), vc = scol ^ G::vswizzle(r);
+            const bool is = (unsigned)page[i] < (unsigned)c.pages;
+            const char* kp = c.k_head(hk) + c.k_at(page[i], slot) + kc * 16;
+            const char* vp = c.v_head(hk) + c.v_at(page[i], slot) + vc * 16;
+            const bool kl = is && (DP * E == c.dim * E || kc * 16 < c.dim * E), vl = is && (DP * E == c.dim * E || vc * 16 < c.dim * E);
+            if (scol == 0) there[t % RING][r] = is;
+            full = full && __any(kl) && __any(vl);      // both loads are made
+            if (kl) __builtin_amdgcn_global_load_lds((gbl_void*)kp, (lds_void*)(K + i * NT * 16), 16, 0, 0);
+            if (vl) __builtin_amdgcn_global_load_lds((gbl_void*)vp, (lds_void*)(V + i * NT * 16), 16, 0, 0);
+            else *(float4*)(V + i * NT * 16 + lane * 16) = make_float4(0.f, 0.f, 0.f, 0.f);
         }
-        return s;
     };
-    auto put = [&](int t, Stage& s, const int (&pg)[PER]) {
-        unsigned char* K = smem + (t & 1) * G::STAGE;
-        unsigned char* V = K + KT * G::KPITCH;
-        // a tile that some row of the workgroup sees in part: values that are not finite are set aside
-        const bool part = (a.causal && t * KT + KT - 1 > pmin) || (a.window && t * KT <= pmax - a.window);
+    // Before tile t: its V and the K of the next one have come, for all waves. `left`: the tile after that may still come.
+    auto arrive = [&](bool left) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (left) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * PER) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // A tile that some row of the workgroup sees in part: values that are not finite are set aside.
+    auto clean = [&](int t) {
+        if (!((a.causal && t * KT + KT - 1 > pmin) || (a.window && t * KT <= pmax - a.window))) return;
+        unsigned char* V = V0 + (t % RING) * G::TILE + tid * 16;
+        bool bad = false;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int r = srow + i * RSTEP;
-            if (scol == 0) there[t & 1][r] = pg[i] >= 0;
-            if (part) {
-                bool bad = false;
-                s.v[i] = make_float4(finite_word<T>(s.v[i].x, bad), finite_word<T>(s.v[i].y, bad),
-                                     finite_word<T>(s.v[i].z, bad), finite_word<T>(s.v[i].w, bad));
-                if (bad) odd[t & 1] = t;
-            }
-            *(float4*)(K + r * G::KPITCH + G::kpiece(r, scol) * 16) = s.k[i];
-            *(float4*)(V + r * G::VPITCH + scol * 16) = s.v[i];
+            const float4 x = *(const float4*)(V + i * NT * 16);
+            *(float4*)(V + i * NT * 16) = make_float4(finite_word<T>(x.x, bad), finite_word<T>(x.y, bad),
+                                                      finite_word<T>(x.z, bad), finite_word<T>(x.w, bad));
         }
+        if (bad) odd[t & 1] = t;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
     };
-    const int tr_row = 4 * h + ((lane & 15) >> 2), tr_col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    // where the lane's fragments lie in a tile
+    const int tr_row = 4 * h + ((lane & 15) >> 2), tr_piece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    const int krow = fr * G::PITCH, kx = (h ^ G::kswizzle(fr)) * 16;
+    int vx[ND], vy[F32 ? 1 : ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+        if constexpr (F32) {
+            vx[d] = 4 * h * G::PITCH + (((8 * d + (fr >> 2)) ^ G::vswizzle(4 * h)) << 4) + (fr & 3) * 4;
+        } else {
+            vx[d] = tr_row * G::PITCH + (((4 * d + tr_piece) ^ G::vswizzle(tr_row)) << 4) + (lane & 1) * 8;
+            vy[d] = (tr_row + 8) * G::PITCH + (((4 * d + tr_piece) ^ G::vswizzle(tr_row + 8)) << 4) + (lane & 1) * 8;
+        }
+    }
 
-    auto compute = [&](int t) {
-        const unsigned char* K = smem + (t & 1) * G::STAGE;
-        const unsigned char* V = K + KT * G::KPITCH;
-        const int j0 = t * KT;
-        f32x16 s[NB];
+    // S^T of tile t
+    auto scores = [&](int t, f32x16 (&s)[NB]) {
+        const unsigned char* K = K0 + (t % RING) * G::TILE + krow;
 #pragma unroll
-        for (int kb = 0; kb < NB; ++kb) {
+        for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
-            const int r = kb * 32 + fr;
 #pragma unroll
-            for (int k = 0; k < NQ; ++k) {
-                const float4 kf = *(const float4*)(K + r * G::KPITCH + G::kpiece(r, 2 * k + h) * 16);
+        for (int k = 0; k < NQ; ++k)
+#pragma unroll
+            for (int kb = 0; kb < NB; ++kb) {
+                const float4 kf = *(const float4*)(K + kb * 32 * G::PITCH + (kx ^ (32 * k)));
                 if constexpr (F32) {
                     s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.x, qf[k].x, s[kb], 0, 0, 0);
                     s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf.y, qf[k].y, s[kb], 0, 0, 0);
@@ -727,11 +762,22 @@ __global__ __launch_bounds__((TileGeom<T, DP>::NW * 64), (TileGeom<T, DP>::NW / 
                     s[kb] = Mma32<T>::mul(*(const typename Mma<T>::frag*)&kf, *(const typename Mma<T>::frag*)&qf[k], s[kb]);
                 }
             }
-        }
-        const unsigned long long here = __ballot(lane < KT && there[t & 1][lane & (KT - 1)]);
+    };
+    auto largest = [&](const f32x16 (&s)[NB]) -> float {
+        float mt = -INFINITY;
+#pragma unroll
+        for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[kb][e]);
+        return mt;
+    };
+    // -inf for the keys that the rows do not see; the rows' largest score, in units of the exponents; mt: this lane's
+    // largest before
+    auto mask = [&](int t, f32x16 (&s)[NB], float mt) -> float {
+        const int j0 = t * KT;
+        const unsigned long long here = __ballot(lane < KT && there[t % RING][lane & (KT - 1)]);
         const bool some = here != (KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1);
-        const bool edge = some || (a.causal && j0 + KT - 1 > wmin) || (a.window && j0 <= wmax - a.window);
-        if (edge) {
+        if (some || (a.causal && j0 + KT - 1 > wmin) || (a.window && j0 <= wmax - a.window)) {
             asm volatile("" ::: "memory");    // a branch of its own: not folded into every tile
 #pragma unroll
             for (int kb = 0; kb < NB; ++kb) {
@@ -746,98 +792,160 @@ __global__ __launch_bounds__((TileGeom<T, DP>::NW * 64), (TileGeom<T, DP>::NW / 
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[kb][e] = bits & (1u << kappa(e)) ? s[kb][e] : -INFINITY;
             }
+            mt = largest(s);
         }
-        // m is the maximum at its last change, in units of the products: a score may pass it by 2^8 before all is rescaled
+        return xor32_max(mt) * a.scale_log2;
+    };
+    // tiles of which some row of the wave sees some key: [t0, tw)
+    const int tw = idle ? t0 : a.causal ? min(t1, wmax < 0 ? t0 : wmax / KT + 1) : t1;
+
+    // A wave's loop is one tile ahead with the scores: the products of tile t + 1 run under the exponentials of tile t. The
+    // loads are three tiles ahead, the page ids four; a wave waits for its loads in the order it made them, so the ids go
+    // before the loads of the same turn.
+    if (tid < 2) odd[tid] = -1;
+    if (DP > c.dim)      // places behind the head's dims are not loaded: zeros
+        for (int i = tid; i < G::LDS / 16; i += NT) ((float4*)smem)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    __syncthreads();
+    if (t0 < t1) {
+        f32x16 sa[NB], sb[NB];
         float mt = -INFINITY;
-#pragma unroll
-        for (int kb = 0; kb < NB; ++kb)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[kb][e]);
-        mt = xor32_max(mt) * a.scale_log2;
-        if (__any(mt > m + 8.f)) {
-            const float mn = fmaxf(m, mt), corr = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
-            l *= corr;
-#pragma unroll
-            for (int d = 0; d < ND; ++d)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[d][e] *= corr;
-            m = mn;
+        pages(t0);
+        bring(t0);
+        pages(t0 + 1);
+        if (t0 + 1 < t1) bring(t0 + 1);
+        pages(t0 + 2);
+        if (t0 + 2 < t1) bring(t0 + 2);
+        pages(t0 + 3);
+        arrive(false);
+        if (t0 < tw) {
+            scores(t0, sa);
+            mt = mask(t0, sa, largest(sa));
         }
-        const float mu = m == -INFINITY ? 0.f : m;
+        bool ahead = false;              // the last 2 PER loads may still be on their way
+        auto next = [&](int t) {
+            if (t > t0) arrive(ahead);
+            const bool more = t + 3 < t1;
+            int now[PER];
 #pragma unroll
-        for (int kb = 0; kb < NB; ++kb)
+            for (int i = 0; i < PER; ++i) now[i] = page[i];
+            pages(t + 4);
+            int then[PER];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                s[kb][e] = __builtin_amdgcn_exp2f(fmaf(s[kb][e], a.scale_log2, -mu));
-                l += s[kb][e];
-            }
-        if constexpr (F32) {
+            for (int i = 0; i < PER; ++i) { then[i] = page[i]; page[i] = now[i]; }
+            if (more) bring(t + 3);
 #pragma unroll
-            for (int kb = 0; kb < NB; ++kb)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float* vr = (const float*)(V + (kb * 32 + kappa(e) + 4 * h) * G::VPITCH) + fr;
-#pragma unroll
-                    for (int d = 0; d < ND; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vr[32 * d], s[kb][e], o[d], 0, 0, 0);
-                }
-        } else {
-#pragma unroll
-            for (int st = 0; st < KT / 16; ++st) {
-                Vec8<T> pb;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) pb.x[j] = from_f<T>(s[st >> 1][8 * (st & 1) + j]);
-                const unsigned char* vp = V + (16 * st + tr_row) * G::VPITCH + tr_col * 2;
-#pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    const v4i16 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vp + 64 * d));
-                    const v4i16 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vp + 8 * G::VPITCH + 64 * d));
-                    const v8i16 va = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-                    o[d] = Mma32<T>::mul(*(const typename Mma<T>::frag*)&va, *(const typename Mma<T>::frag*)&pb, o[d]);
-                }
-            }
-        }
-        if (odd[t & 1] == t) {     // values set aside reach the rows that see them (whatever their weight), and no others
-            asm volatile("" ::: "memory");
-            for (int kr = 0; kr < KT; ++kr) {
-                if (!((here >> kr) & 1)) continue;
-                const int j = j0 + kr;
-                if (a.causal && j > pos) continue;
-                if (a.window && j <= pos - a.window) continue;
-                const int pi = c.by_page.div(j);
-                const T* vr = (const T*)(c.v + ((long long)c.table[b * c.table_stride + pi] * c.vs[0] +
-                                                (long long)(j - pi * c.page) * c.vs[1] + (long long)hk * c.vs[2]) * E);
-                int d0 = 4 * h;
-                asm volatile("" : "+v"(d0));       // nothing of this is kept ready for every tile
+            for (int i = 0; i < PER; ++i) page[i] = then[i];
+            ahead = more && full;
+            clean(t);
+        };
+        // tile t with the scores s, the next ones into sn
+        auto step = [&](int t, f32x16 (&s)[NB], f32x16 (&sn)[NB]) {
+            next(t);
+            // m is the maximum at its last change: a score may pass it by 2^8 before all is rescaled
+            if (__any(mt > m + 8.f)) {
+                asm volatile("" ::: "memory");
+                const float mn = fmaxf(m, mt), corr = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+                l *= corr;
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
 #pragma unroll
-                    for (int i = 0; i < 16; i += 4) add_odd<T>(vr, d0 + 32 * d + kappa(i), c.dim, o[d], i);
+                    for (int e = 0; e < 16; ++e) o[d][e] *= corr;
+                m = mn;
             }
-        }
-    };
-
-    // tile t + 1 comes into registers under tile t's products and is written to the other buffer after them; the page
-    // ids of the tile after it are on their way by then
-    if (tid < 2) odd[tid] = -1;
-    if (t0 < t1) {
-        int pg[PER];
-        pages(t0);
-        Stage s = fetch(t0);
+            const float mu = m == -INFINITY ? 0.f : m;
+            float ma = -INFINITY;
+            const unsigned char* V = V0 + (t % RING) * G::TILE;
+            if constexpr (F32) {
+                scores(t + 1, sn);
+                float p[16 * NB];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) pg[i] = page[i];
-        pages(t0 + 1);
-        __syncthreads();
-        put(t0, s, pg);
-        __syncthreads();
-        for (int t = t0; t < t1; ++t) {
-            s = fetch(t + 1);
+                for (int e = 0; e < 16 * NB; ++e) {
+                    p[e] = __builtin_amdgcn_exp2f(fmaf(s[e >> 4][e & 15], a.scale_log2, -mu));
+                    l += p[e];
+                }
 #pragma unroll
-            for (int i = 0; i < PER; ++i) pg[i] = page[i];
-            pages(t + 2);
-            if (!(a.causal && t * KT > wmax) && !idle) compute(t);
-            if (t + 1 < t1) put(t + 1, s, pg);
-            __syncthreads();
+                for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const unsigned char* x = V + (kb * 32 + kappa(e)) * G::PITCH;
+#pragma unroll
+                        for (int d = 0; d < ND; ++d)
+                            o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(*(const float*)(x + vx[d]), p[16 * kb + e], o[d], 0, 0, 0);
+                    }
+                ma = largest(sn);
+            } else {
+                // in steps that stay in this order: a product of the next scores with its share of the exponentials,
+                // then a product with the values and its share of the next maximum; fragments come AK and AV steps ahead
+                constexpr int NS = NQ * NB, NP = ND * KT / 16, AK = 2, AV = 2;
+                const unsigned char* K = K0 + ((t + 1) % RING) * G::TILE + krow;
+                auto kread = [&](int i) {
+                    return *(const float4*)(K + (i % NB) * 32 * G::PITCH + (kx ^ (32 * (i / NB))));
+                };
+                auto vread = [&](int i) {
+                    const unsigned char* vp = V + 16 * (i / ND) * G::PITCH;
+                    const v4i16 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vp + vx[i % ND]));
+                    const v4i16 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vp + vy[i % ND]));
+                    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+                };
+                Vec8<T> pb[2 * NB];
+                float4 kf[AK + 1];
+                v8i16 vf[AV + 1];
+#pragma unroll
+                for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) sn[kb][e] = 0.f;
+#pragma unroll
+                for (int i = 0; i < AK; ++i) kf[i] = kread(i);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < NS; ++i) {
+                    if (i + AK < NS) kf[(i + AK) % (AK + 1)] = kread(i + AK);
+                    if (i + AV >= NS) vf[i + AV - NS] = vread(i + AV - NS);
+                    sn[i % NB] = Mma32<T>::mul(*(const typename Mma<T>::frag*)&kf[i % (AK + 1)],
+                                               *(const typename Mma<T>::frag*)&qf[i / NB], sn[i % NB]);
+#pragma unroll
+                    for (int e = 16 * NB * i / NS; e < 16 * NB * (i + 1) / NS; ++e) {
+                        const float x = __builtin_amdgcn_exp2f(fmaf(s[e >> 4][e & 15], a.scale_log2, -mu));
+                        l += x;
+                        pb[e >> 3].x[e & 7] = from_f<T>(x);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int i = 0; i < NP; ++i) {
+                    if (i + AV < NP) vf[(i + AV) % (AV + 1)] = vread(i + AV);
+                    o[i % ND] = Mma32<T>::mul(*(const typename Mma<T>::frag*)&vf[i % (AV + 1)],
+                                              *(const typename Mma<T>::frag*)&pb[i / ND], o[i % ND]);
+#pragma unroll
+                    for (int e = 16 * NB * i / NP; e < 16 * NB * (i + 1) / NP; ++e) ma = fmaxf(ma, sn[e >> 4][e & 15]);
+                    asm volatile("" : "+v"(ma));         // here, not where it is used
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            if (odd[t & 1] == t) {   // values set aside reach the rows that see them (whatever their weight), and no others
+                asm volatile("" ::: "memory");
+                for (int k = 0; k < KT; ++k) {
+                    const int j = t * KT + k;
+                    if (!there[t % RING][k] || (a.causal && j > pos) || (a.window && j <= pos - a.window)) continue;
+                    const int pi = c.by_page.div(j);
+                    const T* x = (const T*)(c.v_head(hk) + c.v_at(page_of(c, b, pi), j - pi * c.page));
+                    int d0 = 4 * h;
+                    asm volatile("" : "+v"(d0));       // nothing of this is kept ready for every tile
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4) add_odd<T>(x, d0 + 32 * d + kappa(i), c.dim, o[d], i);
+                }
+            }
+            if (t + 1 < tw) mt = mask(t + 1, sn, ma);
+        };
+        int t = t0;
+        while (t < tw) {
+            step(t++, sa, sb);
+            if (t >= tw) break;
+            step(t++, sb, sa);
         }
+        for (; t < t1; ++t) next(t);     // the other waves' tiles
     }
     l = xor32_add(l);
     if (w0 + fr >= nrows) return;
@@ -937,8 +1045,8 @@ template <typename T, int DP>
 hipError_t run_attention(const PagedAttnArgs& a, hipStream_t st) {
     using R = DecGeom<T, DP>;
     using G = TileGeom<T, DP>;
-    static_assert(R::LDS <= 150 * 1024 && G::LDS <= 150 * 1024, "LDS of a workgroup");
     constexpr bool TILE = sizeof(T) == 2 || DP <= 128;     // as in pfm_paged_attention_plan
+    static_assert(R::LDS <= 150 * 1024 && (!TILE || G::LDS <= 150 * 1024), "LDS of a workgroup");
     const PagedKv& c = a.c;
     hipError_t e = hipSuccess;
     if (a.rows_tiles) {

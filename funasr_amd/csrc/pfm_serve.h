@@ -18,11 +18,11 @@ enum { DT_F16 = 3 };
 struct PfmDevOp { const char* name; const void* p; };
 
 // x / d for 0 <= x < 2^31 by one multiply: m = ceil(2^(32 + s) / d) with s = ceil(log2 d) gives the exact quotient
-// (m < 2^33; the part above 2^32 is added back as x itself, which cannot overflow 64 bits).
+// (m < 2^33; the part above 2^32 is added back as x itself, which cannot overflow 64 bits; d = 1 gives x).
 struct FastDiv {
     uint32_t mul, shift, d;
     __device__ __forceinline__ int div(int x) const {
-        return d == 1 ? x : (int)(((unsigned long long)__umulhi((uint32_t)x, mul) + (uint32_t)x) >> shift);
+        return (int)(((unsigned long long)__umulhi((uint32_t)x, mul) + (uint32_t)x) >> shift);
     }
 };
 static inline FastDiv fast_div(uint32_t d) {
@@ -45,10 +45,11 @@ template <auto KERNEL> hipError_t pfm_allow_lds(int bytes) {
     if (e == hipSuccess) done.fetch_or(bit);
     return e;
 }
-// A batch of sequences whose keys and values lie in pages. Strides count elements; the head dimension is contiguous.
+// A batch of sequences whose keys and values lie in pages. Strides count 16-byte pieces (so that an offset takes one
+// 32 x 32 -> 64 bit multiply-add per stride); the head dimension is contiguous.
 struct PagedKv {
     char *k, *v;                        // pages
-    long long ks[3], vs[3];             // strides of page, slot in the page, head
+    uint32_t ks[3], vs[3];              // strides of page, slot in the page, head
     long long pages;
     const int* table;                   // [batch][table_stride]: page of key positions P i .. P i + P - 1
     long long table_stride;
@@ -57,6 +58,16 @@ struct PagedKv {
     FastDiv by_page;
     const int* kv_len;                  // [batch]: keys of the sequence, this call's new tokens included
     const int* cu_q;                    // [batch + 1]: first row of each sequence's new tokens, or null: one token each
+
+    // Byte offsets of head 0 of a slot.
+    __device__ __forceinline__ unsigned long long k_at(int pg, int slot) const {
+        return ((unsigned long long)(uint32_t)pg * ks[0] + (unsigned long long)(uint32_t)slot * ks[1]) * 16;
+    }
+    __device__ __forceinline__ unsigned long long v_at(int pg, int slot) const {
+        return ((unsigned long long)(uint32_t)pg * vs[0] + (unsigned long long)(uint32_t)slot * vs[1]) * 16;
+    }
+    __device__ __forceinline__ char* k_head(int h) const { return k + (unsigned long long)(uint32_t)h * ks[2] * 16; }
+    __device__ __forceinline__ char* v_head(int h) const { return v + (unsigned long long)(uint32_t)h * vs[2] * 16; }
 
     // The sequence's keys: never more than its table row can name.
     __device__ __forceinline__ int len(int b) const {

@@ -61,7 +61,14 @@ int check_cache(const char* fn, const pfm_paged_kv* c, PagedKv& o) {
     }
     o.k = (char*)c->k;
     o.v = (char*)c->v;
-    for (int i = 0; i < 3; ++i) { o.ks[i] = c->k_stride[i]; o.vs[i] = c->v_stride[i]; }
+    const int per = 16 / elem_bytes(c->dtype);
+    for (int i = 0; i < 3; ++i) {
+        if (c->k_stride[i] / per > 0xffffffffll || c->v_stride[i] / per > 0xffffffffll)
+            return fail(fn, PFM_E_ARG, "strides of the pages must stay under 64 GiB");
+        o.ks[i] = (uint32_t)(c->k_stride[i] / per);
+        o.vs[i] = (uint32_t)(c->v_stride[i] / per);
+    }
+    if (c->pages > 0x7fffffffll) return fail(fn, PFM_E_ARG, "at most 2^31 - 1 pages");
     o.pages = c->pages;
     o.table = c->block_table;
     o.table_stride = c->table_stride;
@@ -125,7 +132,7 @@ int pfm_op_kv_append(void* stream, const pfm_paged_kv* cache, const pfm_rows* k,
             if (!apart(cache->tokens, a.qo.ts, a.c.dim) || !apart(q_heads, a.qo.hs, a.c.dim))
                 return fail(fn, PFM_E_ARG, "q_out overlaps itself");
         }
-        for (const long long* st : {a.c.ks, a.c.vs})
+        for (const int64_t* st : {cache->k_stride, cache->v_stride})
             if (!apart(a.c.pages, st[0], a.c.dim) || !apart(a.c.page, st[1], a.c.dim) || !apart(a.c.heads, st[2], a.c.dim))
                 return fail(fn, PFM_E_ARG, "the pages overlap themselves");
         a.q_heads = q_heads;
