@@ -5,6 +5,8 @@
 // kv_len[b] - (cu_q[b + 1] - cu_q[b]) + (n - cu_q[b]); position t lies in slot t % P of page block_table[b][t / P].
 // A page id outside [0, pages) names no page: nothing is written there and its keys are not seen, so no table
 // content can reach memory outside the pages.
+#include <math.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -227,9 +229,9 @@ __device__ __forceinline__ void add_odd(const T* row, int dd, int dim, V& o, int
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 constexpr int DEC_W = 4;      // waves of a workgroup; each runs over key blocks of its own
-template <typename T, int DP> struct DecGeom {
+template <typename T, int DP, int NTILES> struct DecGeom {
     static constexpr int PITCH = DP * sizeof(T) + (sizeof(T) == 2 ? 32 : 16);   // rows of V: no bank met twice
-    static constexpr int NT = sizeof(T) * DP > 512 ? 1 : 2;                    // 16-key tiles of a block: what registers hold
+    static constexpr int NT = NTILES;                                          // 16-key tiles of a block
     static constexpr int KB = 16 * NT;
     static constexpr int WAVE = KB * PITCH;
     static constexpr int MERGE = DEC_W * 16 * (DP + 4) * 4;                     // overlays the V blocks at the end
@@ -275,9 +277,9 @@ __device__ __forceinline__ bool find_tile(const PagedKv& c, int group, int rows,
 
 // One workgroup = 16 query rows of one sequence and kv head; its waves take key blocks in turn, each with its own V
 // block in LDS and no barrier until the waves' results are joined.
-template <typename T, int DP>
+template <typename T, int DP, int NTILES>
 __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a) {
-    using G = DecGeom<T, DP>;
+    using G = DecGeom<T, DP, NTILES>;
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int ND = DP / 16;
     constexpr int E = sizeof(T), NT = G::NT, KB = G::KB;
@@ -592,8 +594,9 @@ typedef const __attribute__((address_space(1))) void gbl_void;
 
 template <typename T, int DP> struct TileGeom {
     static constexpr int E = sizeof(T);
-    static constexpr int NW = DP > 128 ? 4 : 8;            // waves: 256 registers each suffice up to 128 dims
-    static constexpr int ROWS = NW * 32;
+    static constexpr int NW = 8;
+    static constexpr int HALVES = DP > 128 ? 2 : 1;        // 256 registers hold the sums of 128 dims: two waves share 32 rows
+    static constexpr int ROWS = NW * 32 / HALVES;
     static constexpr int KT = E == 2 && DP <= 128 ? 64 : 32;   // keys of a tile
     static constexpr int PITCH = DP * E;                   // a row of K or V
     static constexpr int CPR = PITCH / 16;                 // its 16-byte pieces
@@ -611,10 +614,10 @@ template <typename T, int DP> struct TileGeom {
 };
 
 template <typename T, int DP>
-__global__ __launch_bounds__((TileGeom<T, DP>::NW * 64), (TileGeom<T, DP>::NW / 4)) void paged_tile_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__((TileGeom<T, DP>::NW * 64), 2) void paged_tile_kernel(PagedAttnArgs a) {
     using G = TileGeom<T, DP>;
     constexpr bool F32 = sizeof(T) == 4;
-    constexpr int E = sizeof(T), KT = G::KT, NB = KT / 32, ND = DP / 32, NT = G::NW * 64;
+    constexpr int E = sizeof(T), KT = G::KT, NB = KT / 32, ND = DP / 32 / G::HALVES, NT = G::NW * 64;
     constexpr int NQ = DP * E / 32;                          // 16-byte pieces of a query row that a lane holds
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     __shared__ unsigned char there[G::RING][KT];                 // a tile's keys that exist
@@ -633,7 +636,7 @@ __global__ __launch_bounds__((TileGeom<T, DP>::NW * 64), (TileGeom<T, DP>::NW / 
     const int row0 = tile * G::ROWS, row1 = min(row0 + G::ROWS, nrows) - 1;
     const int pmin = base + a.by_group.div(row0), pmax = base + a.by_group.div(row1);
     // this wave's rows; -1 rows: none
-    const int w0 = row0 + wid * 32, w1 = min(w0 + 32, nrows) - 1;
+    const int w0 = row0 + wid / G::HALVES * 32, w1 = min(w0 + 32, nrows) - 1, dim0 = wid % G::HALVES * ND * 32;
     const bool idle = w0 >= nrows;
     const int wmin = idle ? 0 : base + a.by_group.div(w0), wmax = idle ? -1 : base + a.by_group.div(w1);
     const int row = min(w0 + fr, nrows - 1), place = a.by_group.div(row), head = hk * a.group + row - place * a.group;
@@ -734,10 +737,10 @@ __global__ __launch_bounds__((TileGeom<T, DP>::NW * 64), (TileGeom<T, DP>::NW / 
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
         if constexpr (F32) {
-            vx[d] = 4 * h * G::PITCH + (((8 * d + (fr >> 2)) ^ G::vswizzle(4 * h)) << 4) + (fr & 3) * 4;
+            vx[d] = 4 * h * G::PITCH + (((dim0 / 4 + 8 * d + (fr >> 2)) ^ G::vswizzle(4 * h)) << 4) + (fr & 3) * 4;
         } else {
-            vx[d] = tr_row * G::PITCH + (((4 * d + tr_piece) ^ G::vswizzle(tr_row)) << 4) + (lane & 1) * 8;
-            vy[d] = (tr_row + 8) * G::PITCH + (((4 * d + tr_piece) ^ G::vswizzle(tr_row + 8)) << 4) + (lane & 1) * 8;
+            vx[d] = tr_row * G::PITCH + (((dim0 / 8 + 4 * d + tr_piece) ^ G::vswizzle(tr_row)) << 4) + (lane & 1) * 8;
+            vy[d] = (tr_row + 8) * G::PITCH + (((dim0 / 8 + 4 * d + tr_piece) ^ G::vswizzle(tr_row + 8)) << 4) + (lane & 1) * 8;
         }
     }
 
@@ -929,7 +932,7 @@ __global__ __launch_bounds__((TileGeom<T, DP>::NW * 64), (TileGeom<T, DP>::NW / 
                     if (!there[t % RING][k] || (a.causal && j > pos) || (a.window && j <= pos - a.window)) continue;
                     const int pi = c.by_page.div(j);
                     const T* x = (const T*)(c.v_head(hk) + c.v_at(page_of(c, b, pi), j - pi * c.page));
-                    int d0 = 4 * h;
+                    int d0 = dim0 + 4 * h;
                     asm volatile("" : "+v"(d0));       // nothing of this is kept ready for every tile
 #pragma unroll
                     for (int d = 0; d < ND; ++d)
@@ -957,7 +960,7 @@ __global__ __launch_bounds__((TileGeom<T, DP>::NW * 64), (TileGeom<T, DP>::NW / 
         for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
-                const int dd = 32 * d + kappa(e) + 4 * h;
+                const int dd = dim0 + 32 * d + kappa(e) + 4 * h;
                 if (dd >= c.dim) continue;
                 T y[4];
 #pragma unroll
@@ -972,10 +975,10 @@ __global__ __launch_bounds__((TileGeom<T, DP>::NW * 64), (TileGeom<T, DP>::NW / 
         for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
-                const int dd = 32 * d + kappa(e) + 4 * h;
+                const int dd = dim0 + 32 * d + kappa(e) + 4 * h;
                 if (dd < c.dim) *(f32x4*)(dst + dd) = f32x4{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
             }
-        if (h == 0) { a.part_ml[2 * pr] = m; a.part_ml[2 * pr + 1] = l; }
+        if (h == 0 && dim0 == 0) { a.part_ml[2 * pr] = m; a.part_ml[2 * pr + 1] = l; }
     }
 }
 
@@ -1041,21 +1044,36 @@ template <typename T> hipError_t run_join(const PagedAttnArgs& a, long long tile
     return hipSuccess;
 }
 
+template <typename T, int DP, int NTILES> hipError_t run_rows(const PagedAttnArgs& a, hipStream_t st) {
+    using R = DecGeom<T, DP, NTILES>;
+    static_assert(R::LDS <= 150 * 1024, "LDS of a workgroup");
+    const PagedKv& c = a.c;
+    hipError_t e = pfm_allow_lds<paged_rows_kernel<T, DP, NTILES>>(R::LDS);
+    if (e != hipSuccess) return e;
+    paged_rows_kernel<T, DP, NTILES><<<dim3((unsigned)(a.rows_tiles * c.heads), a.splits), DEC_W * 64, R::LDS, st>>>(a);
+    PFM_LAUNCH_CHECK();
+    if (a.splits == 1) return hipSuccess;
+    const int per = c.cu_q ? 16 : std::min(16, a.group);     // a sequence's rows where they are known
+    return run_join<T>(a, c.cu_q ? a.rows_tiles : (long long)c.batch * ((a.group + per - 1) / per), per, 0, a.rows_upto,
+                       a.splits, st);
+}
 template <typename T, int DP>
 hipError_t run_attention(const PagedAttnArgs& a, hipStream_t st) {
-    using R = DecGeom<T, DP>;
     using G = TileGeom<T, DP>;
     constexpr bool TILE = sizeof(T) == 2 || DP <= 128;     // as in pfm_paged_attention_plan
-    static_assert(R::LDS <= 150 * 1024 && (!TILE || G::LDS <= 150 * 1024), "LDS of a workgroup");
+    static_assert(!TILE || G::LDS <= 150 * 1024, "LDS of a workgroup");
     const PagedKv& c = a.c;
     hipError_t e = hipSuccess;
     if (a.rows_tiles) {
-        if ((e = pfm_allow_lds<paged_rows_kernel<T, DP>>(R::LDS)) != hipSuccess) return e;
-        paged_rows_kernel<T, DP><<<dim3((unsigned)(a.rows_tiles * c.heads), a.splits), DEC_W * 64, R::LDS, st>>>(a);
-        PFM_LAUNCH_CHECK();
-        const int per = c.cu_q ? 16 : std::min(16, a.group);     // a sequence's rows where they are known
-        if (a.splits > 1) e = run_join<T>(a, c.cu_q ? a.rows_tiles : (long long)c.batch * ((a.group + per - 1) / per), per,
-                                          0, a.rows_upto, a.splits, st);
+        // 32-bit heads: blocks of 32 keys leave a SIMD one wave beyond 64 dims, blocks of 16 two (34 caches of 8230 keys
+        // and 96 dims: 143 -> 88 us); short spans take the longer block all the same (64 streams over 70 keys: 16 us, 19
+        // with 16). Beyond 128 dims it does not fit the registers.
+        if constexpr (sizeof(T) == 4 && DP > 64) {
+            if (DP > 128 || !a.short_span) e = run_rows<T, DP, 1>(a, st);
+            else if constexpr (DP <= 128) e = run_rows<T, DP, 2>(a, st);
+        } else {
+            e = run_rows<T, DP, 2>(a, st);
+        }
         if (e != hipSuccess) return e;
     }
     if constexpr (TILE) if (a.tiles) {
@@ -1118,7 +1136,21 @@ void pfm_paged_attention_plan(int dtype, PagedAttnArgs& a) {
         return a.window ? std::min<long long>(max_kv, (long long)a.window + rows + (a.causal ? 0 : rows == 16 ? std::min(a.rows_upto, c.tokens) : c.tokens)) : max_kv;
     };
     a.splits = parts(a.rows_tiles, seen(16), 2048, 256);
-    a.tile_splits = parts(a.tiles, seen(tile_rows), 256, 512);
+    a.short_span = seen(16) <= 128;
+    // The tile kernel has one workgroup per CU at a time. Split into n parts, its row tiles take so many turns of the 256
+    // CUs, each as long as a part and what a part costs beside its keys; the parts' sums are written and read once more.
+    // Measured at 128 dims: 2.3 us a tile of 64 keys in 16 bits, 7 us one of 32 in 32 bits, 3 us beside, 4 us the join.
+    a.tile_splits = 1;
+    if (a.tiles) {
+        const double wide = c.dim <= 64 ? 0.5 : c.dim <= 128 ? 1.0 : 1.5, units = (double)a.tiles * c.heads;
+        const double tile_us = (dtype == DT_F32 ? 7.0 : 2.3) * wide, n_tiles = seen(tile_rows) / (dtype == DT_F32 ? 32.0 : 64.0);
+        double best = 1e30;
+        for (int n = 1; n <= 64 && n <= n_tiles / 2 + 1; ++n) {
+            const double join = n > 1 ? 4.0 + units * tile_rows * c.dim * 8.0 * n / 4e6 : 0.0;
+            const double us = ceil(units * n / 256) * (ceil(n_tiles / n) * tile_us + 3.0) + join;
+            if (us < best) { best = us; a.tile_splits = n; }
+        }
+    }
 }
 hipError_t pfm_paged_attention(int dtype, const PagedAttnArgs& a, hipStream_t st) {
     if (dtype == DT_F32) return run_attention<float>(a, st);

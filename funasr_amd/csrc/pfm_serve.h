@@ -109,6 +109,7 @@ struct PagedAttnArgs {
     int rows_upto;                      // sequences of at most so many query rows go to the rows kernel
     long long rows_tiles, tiles;        // row tiles of the rows and of the tile kernel at most
     int splits, tile_splits;            // workgroups that share one row tile's keys
+    bool short_span;                    // a row tile of the rows kernel sees at most 128 keys
     float* part;                        // with splits: [splits][tokens * q_heads] rows of dim sums, then max and sum
     float* part_ml;
 };
