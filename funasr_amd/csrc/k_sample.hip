@@ -468,6 +468,16 @@ __device__ __forceinline__ u64 nucleus(const Setting& g, u64 total) {
     return want < 1.0 ? 1 : want >= (double)total ? total : (u64)want;
 }
 
+// The step below which the tokens are that may be kept (a bin or two more than the bound, for the steps' own rounding).
+// kth_bin: the bin that the k-th largest of some tokens is in.
+__device__ __forceinline__ float candidate_limit(const Setting& g, int V, int kth_bin) {
+    float limit = (float)BINS;
+    if (g.by_k) limit = fminf(limit, kth_bin + 1.f);
+    else if (g.by_p) limit = fminf(limit, logf((float)V / (1.f - g.top_p)) * (1.0001f * BINS / SPAN) + 2.f);
+    if (g.by_min && !(g.by_k && g.by_p)) limit = fminf(limit, -logf(fminf(g.min_p, 1.f)) * (1.0001f * BINS / SPAN) + 2.f);
+    return limit;
+}
+
 enum { DONE, SUMS, NARROW, WIDE, FULL, INFS };  // how a row is done; DONE: by its maxima alone
 struct RowWs {                           // one per row
     u64 list[CAND];
@@ -576,9 +586,8 @@ __global__ __launch_bounds__(CT, 4) void sample_scan_kernel(SampleArgs a, Plan p
     const Row r = g.r;
     load_exps(s.exp_table, tid, CT);
 
-    // candidates: steps(x) < limit (a bin or two more than the bound, for the steps' own rounding)
     const int parts = p.chunks * p.groups;
-    float limit = (float)BINS;
+    int kth = BINS;
     if (g.by_k) {
         unsigned* n = (unsigned*)s.data;
         for (int i = tid; i < BINS; i += CT) n[i] = 0;
@@ -589,11 +598,9 @@ __global__ __launch_bounds__(CT, 4) void sample_scan_kernel(SampleArgs a, Plan p
         }
         __syncthreads();
         u64 before;
-        limit = fminf(limit, find_bin<CW>(n, s.wsum, &s.i0, &s.b0, tid, g.top_k, before) + 1.f);
-    } else if (g.by_p) {
-        limit = fminf(limit, logf((float)a.vocab / (1.f - g.top_p)) * (1.0001f * BINS / SPAN) + 2.f);
+        kth = find_bin<CW>(n, s.wsum, &s.i0, &s.b0, tid, g.top_k, before);
     }
-    if (g.by_min && !(g.by_k && g.by_p)) limit = fminf(limit, -logf(fminf(g.min_p, 1.f)) * (1.0001f * BINS / SPAN) + 2.f);
+    const float limit = candidate_limit(g, a.vocab, kth);
     int kind = g.by_k ? NARROW : SUMS;
     if (g.by_p && !g.by_k) {
         int pass = 0;
@@ -819,6 +826,50 @@ __device__ __forceinline__ Cut cuts(A all, int V, const Setting& g, Lds& s, int 
     return cut;
 }
 
+// The end of a row whose n <= CAND candidates are in s.cand; total: all mass where top-p stands alone.
+__device__ __forceinline__ void draw_narrow(const SampleArgs& a, Lds& s, int tid, int b, const Setting& g, int n, u64 total) {
+    if (n <= FEW) {
+        // few: each token's place in the order and the mass ahead of it say whether it is kept
+        u64 rank, before, t;
+        const u64 e = rank_few(s, n, tid, g.r, [&](int i) { return s.cand[i]; }, rank, before);
+        const bool own = tid < 4 * n && !(tid & 3);
+        const u64 y = own ? s.few[tid >> 2].y : 0;
+        bool keep = own && (!g.by_k || rank < (u64)g.top_k);
+        if (g.by_k) block_scan<SW>(keep ? y : 0, s.wsum, tid, total);
+        keep = keep && (!g.by_p || before < nucleus(g, total)) && y >= g.least;
+        block_scan<SW>(keep ? y : 0, s.wsum, tid, total);
+        if (own) s.few[tid >> 2] = make_ulonglong2(e & 0xffffffff, keep ? y : 0);     // index and what is kept
+        __syncthreads();
+        const u64 target = aim(g, total);
+        t = 0;
+        if (tid < 4 * n) over_few(s, n, tid, [&](const ulonglong2& o) { t += o.x < (e & 0xffffffff) ? o.y : 0; });
+        t = four_sum(t);
+        if (keep && t <= target && t + y > target) {
+            a.token[b] = entry_index(e);
+            if (a.prob) a.prob[b] = (float)((double)y / (double)total);
+        }
+        return;
+    }
+    for (int i = tid; i < BINS; i += ST) { s.hist_w[i] = 0; s.hist_n[i] = 0; }
+    __syncthreads();
+    auto all = [&](auto f) {
+        for (int i = tid; i < n; i += ST) f(entry_index(s.cand[i]), entry_value(s.cand[i]));
+    };
+    all([&](int i, float f) {
+        const int bin = bin_of(f, g.r);
+        if (bin >= BINS) return;
+        if (g.by_k) atomicAdd(&s.hist_n[bin], 1u);
+        if (g.by_p) atomicAdd(&s.hist_w[bin], mass(f, g.r, s.exp_table));
+    });
+    __syncthreads();
+    const Cut cut = cuts(all, a.vocab, g, s, tid, nullptr, total);
+    draw_from(a, all, s, tid, b, g, [&](int i, float f) -> u64 {
+        if (!kept(f, i, cut)) return 0;
+        const u64 y = mass(f, g.r, s.exp_table);
+        return y >= g.least ? y : 0;
+    });
+}
+
 // Third, one workgroup per row: the rows that are done, and the WIDE rows' bin.
 template <typename T>
 __global__ __launch_bounds__(ST) void sample_pick_kernel(SampleArgs a, Plan p) {
@@ -883,47 +934,9 @@ __global__ __launch_bounds__(ST) void sample_pick_kernel(SampleArgs a, Plan p) {
         return;
     }
     const int n = (int)n64;
-    if (n <= FEW) {
-        // few: each token's place in the order and the mass ahead of it say whether it is kept
-        u64 rank, before, t;
-        const u64 e = rank_few(s, n, tid, g.r, [&](int i) { return w.list[i]; }, rank, before);
-        const bool own = tid < 4 * n && !(tid & 3);
-        const u64 y = own ? s.few[tid >> 2].y : 0;
-        bool keep = own && (!g.by_k || rank < (u64)g.top_k);
-        if (g.by_k) block_scan<SW>(keep ? y : 0, s.wsum, tid, total);
-        keep = keep && (!g.by_p || before < nucleus(g, total)) && y >= g.least;
-        block_scan<SW>(keep ? y : 0, s.wsum, tid, total);
-        if (own) s.few[tid >> 2] = make_ulonglong2(e & 0xffffffff, keep ? y : 0);     // index and what is kept
-        __syncthreads();
-        const u64 target = aim(g, total);
-        t = 0;
-        if (tid < 4 * n) over_few(s, n, tid, [&](const ulonglong2& o) { t += o.x < (e & 0xffffffff) ? o.y : 0; });
-        t = four_sum(t);
-        if (keep && t <= target && t + y > target) {
-            a.token[b] = entry_index(e);
-            if (a.prob) a.prob[b] = (float)((double)y / (double)total);
-        }
-        return;
-    }
     for (int i = tid; i < n; i += ST) s.cand[i] = w.list[i];
-    for (int i = tid; i < BINS; i += ST) { s.hist_w[i] = 0; s.hist_n[i] = 0; }
     __syncthreads();
-    auto all = [&](auto f) {
-        for (int i = tid; i < n; i += ST) f(entry_index(s.cand[i]), entry_value(s.cand[i]));
-    };
-    all([&](int i, float f) {
-        const int bin = bin_of(f, g.r);
-        if (bin >= BINS) return;
-        if (g.by_k) atomicAdd(&s.hist_n[bin], 1u);
-        if (g.by_p) atomicAdd(&s.hist_w[bin], mass(f, g.r, s.exp_table));
-    });
-    __syncthreads();
-    const Cut cut = cuts(all, a.vocab, g, s, tid, nullptr, total);
-    draw_from(a, all, s, tid, b, g, [&](int i, float f) -> u64 {
-        if (!kept(f, i, cut)) return 0;
-        const u64 y = mass(f, g.r, s.exp_table);
-        return y >= g.least ? y : 0;
-    });
+    draw_narrow(a, s, tid, b, g, n, total);
 }
 
 // Last, one workgroup per row: the WIDE rows' end, and the rows whose candidates did not fit (FULL) from the logits alone.
@@ -985,6 +998,134 @@ __global__ __launch_bounds__(ST) void sample_rest_kernel(SampleArgs a, Plan p) {
     draw(a, p.chunks, p.chunk, x, s, tid, b, g, total, weight);
 }
 
+// Rows of at most SHORT logits, one workgroup each and nothing else: the logits stay in registers, neighbours in a thread.
+constexpr int OWN = 16, SHORT = OWN * ST;
+template <typename T>
+__global__ __launch_bounds__(ST) void sample_short_kernel(SampleArgs a) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    Lds& s = *(Lds*)smem;
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, b = blockIdx.x, V = a.vocab;
+    const T* x = (const T*)a.x + (long long)b * a.ld;
+    const int per = (V + ST - 1) / ST, i0 = tid * per;
+    float v[OWN], mine = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < OWN; ++j) v[j] = j < per && i0 + j < V ? to_f(x[i0 + j]) : -INFINITY;
+    load_exps(s.exp_table, tid, ST);
+    for (int i = tid; i < BINS; i += ST) { s.hist_w[i] = 0; s.hist_n[i] = 0; }
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int j = 0; j < OWN; ++j)
+        if (v[j] > mine) { mine = v[j]; at = i0 + j; }
+    const float m = wave_max(mine);
+    float* wmax = (float*)s.wsum;
+    if (lane == 0) wmax[wid] = m;
+    __syncthreads();
+    float mx = m;
+#pragma unroll
+    for (int w = 0; w < SW; ++w) mx = fmaxf(mx, wmax[w]);
+    if (mx == -INFINITY || is_greedy(a, b)) {
+        // threads are in the vocabulary's order: the first that has the maximum
+        if (tid == 0) s.i0 = 0x7fffffff;
+        __syncthreads();
+        if (mine == mx) atomicMin(&s.i0, at);
+        __syncthreads();
+        if (tid == 0) {
+            a.token[b] = mx == -INFINITY ? -1 : s.i0;
+            if (a.prob) a.prob[b] = mx == -INFINITY ? 0.f : 1.f;
+        }
+        return;
+    }
+    const Setting g = setting(a, b, mx);
+    // a short loop: this workgroup is alone with its row, and unrolled it fetches more code than it saves (16 against 19 us)
+    auto all = [&](auto f) {
+#pragma unroll 1
+        for (int j = 0; j < per; ++j) {
+            float y = v[0];
+#pragma unroll
+            for (int k = 1; k < OWN; ++k) y = k == j ? v[k] : y;
+            if (y > -INFINITY) f(i0 + j, y);
+        }
+    };
+    u64 total, t;
+    const bool inf = mx == INFINITY;      // its tokens share the mass
+    if (!inf && (g.by_k || g.by_p)) {
+        int kth = BINS;
+        if (g.by_k) {
+            if (bin_of(mine, g.r) < BINS) atomicAdd(&s.hist_n[bin_of(mine, g.r)], 1u);
+            __syncthreads();
+            u64 before;
+            kth = find_bin<SW>(s.hist_n, s.wsum, &s.i0, &s.b0, tid, g.top_k, before);
+        }
+        const float from = value_at(candidate_limit(g, V, kth), g.r);
+        if (tid == 0) s.n_list = 0;
+        __syncthreads();
+        u64 z = 0;
+#pragma unroll
+        for (int j = 0; j < OWN; ++j)
+            if (j < per) push(s.cand, s.n_list, CAND, v[j] >= from, i0 + j, v[j]);
+        if (g.by_p && !g.by_k) {
+#pragma unroll
+            for (int j = 0; j < OWN; ++j)
+                if (j < per) z += mass(v[j], g.r, s.exp_table);
+        }
+        block_scan<SW>(z, s.wsum, tid, total);
+        const int n = (int)s.n_list;
+        __syncthreads();
+        if (n <= CAND) {
+            draw_narrow(a, s, tid, b, g, n, total);
+            return;
+        }
+        for (int i = tid; i < BINS; i += ST) s.hist_n[i] = 0;
+        __syncthreads();
+    }
+    Cut cut{0, V};
+    if (inf) {
+        u64 n = 0;
+        all([&](int i, float f) { n += f == INFINITY; });
+        block_scan<SW>(n, s.wsum, tid, total);
+        if (g.by_k) total = min(total, (u64)g.top_k);
+        if (g.by_p) total = max((u64)1, min(total, (u64)ceil((double)g.top_p * (double)total)));
+    } else if (g.by_k || g.by_p) {
+        u64 z = 0;
+        all([&](int i, float f) {
+            const int bin = bin_of(f, g.r);
+            if (bin >= BINS) return;
+            if (g.by_k) atomicAdd(&s.hist_n[bin], 1u);
+            if (g.by_p) {
+                const u64 y = mass(f, g.r, s.exp_table);
+                atomicAdd(&s.hist_w[bin], y);
+                z += y;
+            }
+        });
+        block_scan<SW>(z, s.wsum, tid, total);
+        cut = cuts(all, V, g, s, tid, nullptr, total);
+    }
+    auto weight = [&](int i, float f) -> u64 {
+        if (inf) return f == INFINITY;
+        if (!kept(f, i, cut)) return 0;
+        const u64 y = mass(f, g.r, s.exp_table);
+        return y >= g.least ? y : 0;
+    };
+    u64 w = 0;
+    all([&](int i, float f) { w += weight(i, f); });
+    const u64 to = block_scan<SW>(w, s.wsum, tid, t);
+    if (!inf) total = t;
+    const u64 target = aim(g, total);
+    u64 run = to - w;
+    if (run <= target && to > target) {
+        bool done = false;
+        all([&](int i, float f) {
+            const u64 y = weight(i, f);
+            if (!done && run + y > target) {
+                done = true;
+                a.token[b] = i;
+                if (a.prob) a.prob[b] = (float)((double)y / (double)total);
+            }
+            run += y;
+        });
+    }
+}
+
 // Chunks of at least 2048 elements, as many as give the chip four workgroups per CU, or one more than that.
 Plan plan(int batch, int vocab) {
     Plan p{};
@@ -999,6 +1140,13 @@ Plan plan(int batch, int vocab) {
 
 template <typename T> hipError_t run(const SampleArgs& a, hipStream_t st) {
     static_assert(sizeof(Lds) <= 150 * 1024 && BINS % ST == 0 && BINS % CT == 0 && CHUNKS <= 64, "sizes");
+    if (a.vocab <= SHORT) {
+        const hipError_t e = pfm_allow_lds<sample_short_kernel<T>>(sizeof(Lds));
+        if (e != hipSuccess) return e;
+        sample_short_kernel<T><<<a.batch, ST, sizeof(Lds), st>>>(a);
+        PFM_LAUNCH_CHECK();
+        return hipSuccess;
+    }
     Plan p = plan(a.batch, a.vocab);
     p.rows = (RowWs*)a.ws;
     p.hist = (u64*)(p.rows + a.batch);
@@ -1020,6 +1168,7 @@ template <typename T> hipError_t run(const SampleArgs& a, hipStream_t st) {
 }  // namespace
 
 long long pfm_sample_ws_bytes(int batch, int vocab) {
+    if (vocab <= SHORT) return 0;
     return (long long)batch * (long long)sizeof(RowWs) + (long long)batch * plan(batch, vocab).chunks * BINS * 8;
 }
 hipError_t pfm_sample(int dtype, const SampleArgs& a, hipStream_t st) {

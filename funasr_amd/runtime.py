@@ -214,7 +214,7 @@ def _on_device(torch, device):
     """The call's device as the current one, where it is another (the library launches on the current device)."""
     if device.type != "cuda":
         raise PfmError(f"device tensors expected, got {device}")
-    return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _NO_GUARD if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def _raw_stream(torch, device) -> int:
