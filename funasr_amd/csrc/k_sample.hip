@@ -505,7 +505,7 @@ template <typename T>
 __global__ __launch_bounds__(CT) void sample_max_kernel(SampleArgs a, Plan p) {
     __shared__ float wmax[CW];
     __shared__ int wat[CW];
-    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, c = blockIdx.x, b = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, c = blockIdx.y, b = blockIdx.x;
     const T* x = (const T*)a.x + (long long)b * a.ld;
     const int e0 = min(c * p.chunk, a.vocab), e1 = min(e0 + p.chunk, a.vocab);
     RowWs& w = p.rows[b];
@@ -567,7 +567,7 @@ template <typename T>
 __global__ __launch_bounds__(CT, 4) void sample_scan_kernel(SampleArgs a, Plan p) {
     __shared__ ChunkLds s;
     constexpr int U = sizeof(T);             // loads of 16 logits under way where each becomes a mass: what the registers hold
-    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, c = blockIdx.x, b = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, c = blockIdx.y, b = blockIdx.x;
     const T* x = (const T*)a.x + (long long)b * a.ld;
     const int e0 = min(c * p.chunk, a.vocab), e1 = min(e0 + p.chunk, a.vocab);
     const int q0 = min(e0 + wid * (p.chunk / CW), e1), q1 = min(q0 + p.chunk / CW, e1);    // this wave's part
@@ -664,7 +664,7 @@ __global__ __launch_bounds__(CT, 4) void sample_scan_kernel(SampleArgs a, Plan p
 template <typename T>
 __global__ __launch_bounds__(CT, 4) void sample_edge_kernel(SampleArgs a, Plan p) {
     __shared__ ChunkLds s;
-    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, c = blockIdx.x, b = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, c = blockIdx.y, b = blockIdx.x;
     RowWs& w = p.rows[b];
     if (w.kind != WIDE) return;
     const float mx = row_max(w, p.chunks, lane);
@@ -998,7 +998,7 @@ __global__ __launch_bounds__(ST) void sample_rest_kernel(SampleArgs a, Plan p) {
     draw(a, p.chunks, p.chunk, x, s, tid, b, g, total, weight);
 }
 
-// Rows of at most SHORT logits, one workgroup each and nothing else: the logits stay in registers, neighbours in a thread.
+// Rows of at most SHORT logits, one workgroup each and nothing else: a thread keeps neighbouring logits.
 constexpr int OWN = 16, SHORT = OWN * ST;
 template <typename T>
 __global__ __launch_bounds__(ST) void sample_short_kernel(SampleArgs a) {
@@ -1036,15 +1036,12 @@ __global__ __launch_bounds__(ST) void sample_short_kernel(SampleArgs a) {
         return;
     }
     const Setting g = setting(a, b, mx);
-    // a short loop: this workgroup is alone with its row, and unrolled it fetches more code than it saves (16 against 19 us)
+    // Short loops, for which the logits are indexed in scratch (they stay in the caches): one row of 8404 with top-k and
+    // top-p 50 takes 13 us. Unrolled over registers each loop is code that a lone workgroup fetches once: 18 us.
     auto all = [&](auto f) {
 #pragma unroll 1
-        for (int j = 0; j < per; ++j) {
-            float y = v[0];
-#pragma unroll
-            for (int k = 1; k < OWN; ++k) y = k == j ? v[k] : y;
-            if (y > -INFINITY) f(i0 + j, y);
-        }
+        for (int j = 0; j < per; ++j)
+            if (v[j] > -INFINITY) f(i0 + j, v[j]);
     };
     u64 total, t;
     const bool inf = mx == INFINITY;      // its tokens share the mass
@@ -1060,14 +1057,8 @@ __global__ __launch_bounds__(ST) void sample_short_kernel(SampleArgs a) {
         if (tid == 0) s.n_list = 0;
         __syncthreads();
         u64 z = 0;
-#pragma unroll
-        for (int j = 0; j < OWN; ++j)
-            if (j < per) push(s.cand, s.n_list, CAND, v[j] >= from, i0 + j, v[j]);
-        if (g.by_p && !g.by_k) {
-#pragma unroll
-            for (int j = 0; j < OWN; ++j)
-                if (j < per) z += mass(v[j], g.r, s.exp_table);
-        }
+        all([&](int i, float f) { push(s.cand, s.n_list, CAND, f >= from, i, f); });
+        if (g.by_p && !g.by_k) all([&](int i, float f) { z += mass(f, g.r, s.exp_table); });
         block_scan<SW>(z, s.wsum, tid, total);
         const int n = (int)s.n_list;
         __syncthreads();
@@ -1153,7 +1144,7 @@ template <typename T> hipError_t run(const SampleArgs& a, hipStream_t st) {
     hipError_t e = pfm_allow_lds<sample_pick_kernel<T>>(sizeof(Lds));
     if (e == hipSuccess) e = pfm_allow_lds<sample_rest_kernel<T>>(sizeof(Lds));
     if (e != hipSuccess) return e;
-    const dim3 grid(p.chunks, a.batch);
+    const dim3 grid(a.batch, p.chunks);
     sample_max_kernel<T><<<grid, CT, 0, st>>>(a, p);
     sample_scan_kernel<T><<<grid, CT, 0, st>>>(a, p);
     sample_pick_kernel<T><<<a.batch, ST, sizeof(Lds), st>>>(a, p);
