@@ -982,6 +982,54 @@ __global__ __launch_bounds__((TileGeom<T, DP>::NW * 64), 2) void paged_tile_kern
     }
 }
 
+// The same for rows of few splits, several rows to a workgroup: a group of lanes holds a row's dims, 4 a lane, and goes
+// over its splits, each lane with one split's weight.
+constexpr int FEW_SPLITS = 16, JOIN_TURNS = 4;
+__host__ __device__ __forceinline__ int join_lanes(int dim) { return dim <= 64 ? 16 : dim <= 128 ? 32 : 64; }
+template <typename T>
+__global__ __launch_bounds__(256) void paged_join_few_kernel(PagedAttnArgs a, int per, int over, int upto, int splits) {
+    const PagedKv& c = a.c;
+    const int lanes = join_lanes(c.dim), at = threadIdx.x % lanes, groups = 256 / lanes, own = JOIN_TURNS * groups;
+    const int parts = (per + own - 1) / own;
+    const int unit = blockIdx.x / parts, hk = unit % c.heads;
+    int b, tile, first, end;
+    if (!find_tile(c, a.group, per, over, upto, unit / c.heads, threadIdx.x & 63, b, tile)) return;
+    c.rows(b, first, end);
+    const int in0 = blockIdx.x % parts * own, row1 = min(tile * per + min(per, in0 + own), (end - first) * a.group);
+    const long long nrow = (long long)c.tokens * a.q_heads;
+    const int d0 = at * 4;
+    for (int row = tile * per + in0 + threadIdx.x / lanes; row < row1; row += groups) {
+        const int place = a.by_group.div(row), n = first + place, head = hk * a.group + row - place * a.group;
+        const long long r0 = (long long)n * a.q_heads + head;
+        f32x4 x[FEW_SPLITS];
+#pragma unroll
+        for (int s = 0; s < FEW_SPLITS; ++s) {
+            x[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (s < splits && d0 < c.dim) x[s] = *(const f32x4*)(a.part + (s * nrow + r0) * c.dim + d0);
+        }
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (at < splits) ml = *(const float2*)(a.part_ml + 2 * (at * nrow + r0));
+        float m = ml.x;
+        for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 16));
+        m = __shfl(m, 0, lanes);
+        const float w = __builtin_amdgcn_exp2f(ml.x - (m == -INFINITY ? 0.f : m));
+        float l = ml.y * w;
+        for (int o = 8; o > 0; o >>= 1) l += __shfl_xor(l, o, 16);
+        l = __shfl(l, 0, lanes);
+        f32x4 y = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < FEW_SPLITS; ++s) y += x[s] * __shfl(w, s, lanes);
+        if (d0 >= c.dim) continue;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        T out[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[e] = from_f<T>(l == 0.f ? 0.f : y[e] * inv);
+        char* dst = a.o.p + ((long long)n * a.o.ts + (long long)head * a.o.hs + d0) * (int)sizeof(T);
+        if constexpr (sizeof(T) == 4) *(float4*)dst = *(const float4*)out;
+        else *(float2*)dst = *(const float2*)out;
+    }
+}
+
 // Joins the splits of one query row, one workgroup each: the splits' sums scaled to their common maximum, then divided
 // once. Rows are numbered as the kernel that split them did, `per` to a row tile.
 template <typename T>
@@ -1039,7 +1087,12 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int pe
 
 template <typename T> hipError_t run_join(const PagedAttnArgs& a, long long tiles, int per, int over, int upto, int splits,
                                           hipStream_t st) {
-    paged_join_kernel<T><<<(unsigned)(tiles * a.c.heads * per), 256, 0, st>>>(a, per, over, upto, splits);
+    if (splits <= FEW_SPLITS) {
+        const int own = JOIN_TURNS * 256 / join_lanes(a.c.dim);
+        paged_join_few_kernel<T><<<(unsigned)(tiles * a.c.heads * ((per + own - 1) / own)), 256, 0, st>>>(a, per, over, upto, splits);
+    } else {
+        paged_join_kernel<T><<<(unsigned)(tiles * a.c.heads * per), 256, 0, st>>>(a, per, over, upto, splits);
+    }
     PFM_LAUNCH_CHECK();
     return hipSuccess;
 }
@@ -1124,7 +1177,9 @@ void pfm_paged_attention_plan(int dtype, PagedAttnArgs& a) {
             a.rows_upto = 0;
             a.rows_tiles = 0;
         }
-        a.tiles = rows > 16 ? rows / tile_rows + std::min<long long>(c.batch, rows / 17) : 0;
+        // sequences of more than 16 rows, each with one tile that is not full
+        a.tiles = (rows + std::min<long long>(c.batch, rows / 17) * (tile_rows - 1)) / tile_rows;
+        if (rows <= 16) a.tiles = 0;
     }
     // keys that one row tile sees at most: with a window its first row's reach and the rows' own span
     auto parts = [&](long long units, long long keys, long long fill, long long least) {
@@ -1139,17 +1194,32 @@ void pfm_paged_attention_plan(int dtype, PagedAttnArgs& a) {
     a.short_span = seen(16) <= 128;
     // The tile kernel has one workgroup per CU at a time. Split into n parts, its row tiles take so many turns of the 256
     // CUs, each as long as a part and what a part costs beside its keys; the parts' sums are written and read once more.
-    // Measured at 128 dims: 2.3 us a tile of 64 keys in 16 bits, 7 us one of 32 in 32 bits, 3 us beside, 4 us the join.
+    // Past one turn, tiles of several sequences end apart, and the last turn is taken as half full. Measured at 128 dims:
+    // 2.3 us a tile of 64 keys in 16 bits, 9 us one of 32 in 32 bits, 3 us beside, 4 us the join. 256 new tokens of 64
+    // heads, each with its own cache of 8192 keys: 289 us whole, 182 in 2 parts, 114 in 4, 130 in 8; 8 sequences of 512
+    // tokens over themselves, 32 heads on 8: 61 whole, 109 in 2.
     a.tile_splits = 1;
     if (a.tiles) {
-        const double wide = c.dim <= 64 ? 0.5 : c.dim <= 128 ? 1.0 : 1.5, units = (double)a.tiles * c.heads;
-        const double tile_us = (dtype == DT_F32 ? 7.0 : 2.3) * wide, n_tiles = seen(tile_rows) / (dtype == DT_F32 ? 32.0 : 64.0);
-        double best = 1e30;
-        for (int n = 1; n <= 64 && n <= n_tiles / 2 + 1; ++n) {
-            const double join = n > 1 ? 4.0 + units * tile_rows * c.dim * 8.0 * n / 4e6 : 0.0;
-            const double us = ceil(units * n / 256) * (ceil(n_tiles / n) * tile_us + 3.0) + join;
-            if (us < best) { best = us; a.tile_splits = n; }
-        }
+        // row tiles that have work: as if all sequences were as long as each other
+        const long long per = (rows + c.batch - 1) / c.batch;
+        const double units = (double)std::min<long long>(a.tiles, c.batch * ((per + tile_rows - 1) / tile_rows)) * c.heads;
+        const double wide = c.dim <= 64 ? 0.5 : c.dim <= 128 ? 1.0 : 1.5;
+        const double tile_us = (dtype == DT_F32 ? 9.0 : 2.3) * wide;
+        auto best_of = [&](long long keys, int most) {
+            const double n_tiles = keys / (dtype == DT_F32 ? 32.0 : 64.0);
+            double best = 1e30;
+            int parts = 1;
+            for (int n = 1; n <= most && n <= n_tiles / 2 + 1; ++n) {
+                const double join = n > 1 ? 4.0 + units * tile_rows * c.dim * 8.0 * n / 4e6 : 0.0;
+                const double turns = units * n / 256, ends = c.batch > 1 && turns > 1.0 ? turns + 0.5 : ceil(turns);
+                const double us = ends * (ceil(n_tiles / n) * tile_us + 3.0) + join;
+                if (us < best) { best = us; parts = n; }
+            }
+            return parts;
+        };
+        // (from 2^16 on a launch of the join would not hold all rows, and there is nothing to fill up)
+        a.tile_splits = best_of(max_kv, a.tiles * c.heads < 65536 ? 64 : 1);
+        if (a.window) a.tile_splits = best_of(seen(tile_rows), a.tile_splits);     // the workspace is that of no window
     }
 }
 hipError_t pfm_paged_attention(int dtype, const PagedAttnArgs& a, hipStream_t st) {

@@ -3,7 +3,9 @@
 #include <math.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <string>
+#include <utility>
 
 #include "../../include/pfm.h"
 #include "pfm_serve.h"
@@ -45,6 +47,7 @@ int check_cache(const char* fn, const pfm_paged_kv* c, PagedKv& o) {
     if (!is_dtype(c->dtype)) return fail(fn, PFM_E_ARG, "dtype must be PFM_F32, PFM_BF16 or PFM_F16");
     if (c->batch < 0 || c->tokens < 0 || c->pages < 0 || c->table_width < 0)
         return fail(fn, PFM_E_ARG, "negative size");
+    if (c->batch > 1 << 24 || c->tokens > 1 << 24) return fail(fn, PFM_E_ARG, "batch and tokens must not pass 2^24");
     if (c->page_size < 1 || c->heads < 1 || c->heads > 65535) return fail(fn, PFM_E_ARG, "page_size and heads must be at least 1, heads at most 65535");
     if (c->head_dim < 8 || c->head_dim > 256 || c->head_dim % 8)
         return fail(fn, PFM_E_ARG, "head_dim must be a multiple of 8 up to 256");
@@ -93,8 +96,21 @@ int check_rows(const char* fn, const char* name, const pfm_rows* r, int dtype, R
     return PFM_OK;
 }
 
-// Places that are written must not lie on each other: strides of dimensions longer than one reach past a head.
-bool apart(int64_t extent, int64_t stride, int dim) { return extent < 2 || stride >= dim; }
+// Places that are written must not lie on each other: in the order of their strides, each dimension longer than one
+// steps over all that the ones before it reach.
+bool apart(std::initializer_list<std::pair<int64_t, int64_t>> extent_stride, int dim) {
+    std::pair<int64_t, int64_t> d[3];      // (stride, extent)
+    int n = 0;
+    for (const auto& e : extent_stride)
+        if (e.first > 1) d[n++] = {e.second, e.first};
+    std::sort(d, d + n);
+    __int128 reach = dim;
+    for (int i = 0; i < n; ++i) {
+        if (d[i].first < reach) return false;
+        reach += (__int128)d[i].first * (d[i].second - 1);
+    }
+    return true;
+}
 
 int hip(const char* fn, hipError_t e) { return e == hipSuccess ? PFM_OK : fail(fn, PFM_E_HIP, hipGetErrorString(e)); }
 
@@ -129,11 +145,11 @@ int pfm_op_kv_append(void* stream, const pfm_paged_kv* cache, const pfm_rows* k,
         if (q_heads) {
             TRY(check_rows(fn, "q", q, cache->dtype, a.q));
             TRY(check_rows(fn, "q_out", q_out, cache->dtype, a.qo));
-            if (!apart(cache->tokens, a.qo.ts, a.c.dim) || !apart(q_heads, a.qo.hs, a.c.dim))
+            if (!apart({{cache->tokens, a.qo.ts}, {q_heads, a.qo.hs}}, a.c.dim))
                 return fail(fn, PFM_E_ARG, "q_out overlaps itself");
         }
         for (const int64_t* st : {cache->k_stride, cache->v_stride})
-            if (!apart(a.c.pages, st[0], a.c.dim) || !apart(a.c.page, st[1], a.c.dim) || !apart(a.c.heads, st[2], a.c.dim))
+            if (!apart({{a.c.pages, st[0]}, {a.c.page, st[1]}, {a.c.heads, st[2]}}, a.c.dim))
                 return fail(fn, PFM_E_ARG, "the pages overlap themselves");
         a.q_heads = q_heads;
         a.inv_freq = inv_freq;
@@ -178,7 +194,7 @@ int pfm_op_paged_attention(void* stream, const pfm_paged_kv* cache, const pfm_ro
         if (cache->batch == 0 || cache->tokens == 0) return PFM_OK;
         TRY(check_rows(fn, "q", q, cache->dtype, a.q));
         TRY(check_rows(fn, "out", out, cache->dtype, a.o));
-        if (!apart(cache->tokens, a.o.ts, a.c.dim) || !apart(q_heads, a.o.hs, a.c.dim))
+        if (!apart({{cache->tokens, a.o.ts}, {q_heads, a.o.hs}}, a.c.dim))
             return fail(fn, PFM_E_ARG, "out overlaps itself");
         a.q_heads = q_heads;
         a.group = q_heads / cache->heads;
@@ -188,6 +204,9 @@ int pfm_op_paged_attention(void* stream, const pfm_paged_kv* cache, const pfm_ro
         a.causal = causal ? 1 : 0;
         a.window = window;
         pfm_paged_attention_plan(cache->dtype, a);
+        // a launch has under 2^32 threads
+        if ((a.rows_tiles + 2 * a.tiles) * cache->heads >= 1ll << 24)
+            return fail(fn, PFM_E_ARG, "too many sequences, tokens and heads for one call");
         const long long need = attention_ws(a);
         if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
             return fail(fn, PFM_E_ARG, "workspace missing, not aligned to 16 bytes or under pfm_paged_attention_ws_bytes");
@@ -211,7 +230,8 @@ int pfm_op_sample(void* stream, int dtype, const void* logits, int64_t ld, int B
     static const char fn[] = "pfm_op_sample";
     return guarded(fn, [&]() -> int {
         if (!is_dtype(dtype)) return fail(fn, PFM_E_ARG, "dtype must be PFM_F32, PFM_BF16 or PFM_F16");
-        if (B < 0 || V < 1 || V > (1 << 20)) return fail(fn, PFM_E_ARG, "need B >= 0 and 1 <= V <= 2^20");
+        if (B < 0 || B > (1 << 20) || V < 1 || V > (1 << 20))
+            return fail(fn, PFM_E_ARG, "need 0 <= B <= 2^20 and 1 <= V <= 2^20");
         if (ld < V) return fail(fn, PFM_E_ARG, "ld is smaller than V");
         if (B == 0) return PFM_OK;
         if (!logits || !u || !token) return fail(fn, PFM_E_ARG, "null operand");

@@ -104,6 +104,55 @@ def test_bad_sample_refused(kw):
     assert b"pfm_op_sample" in lib.pfm_last_error()
 
 
+def test_window_takes_the_workspace_of_no_window():
+    """pfm_paged_attention_ws_bytes knows no window: with any, the call wants no more."""
+    lib = rt.load_library()
+    rng = np.random.default_rng(3)
+    for _ in range(4000):
+        width, n, heads, b = (int(rng.integers(1, x)) for x in (6000, 9000, 12, 9))
+        c = cache(table_width=width, table_stride=width, tokens=n, heads=heads, batch=b,
+                  head_dim=int(rng.choice([64, 128, 256])), k_stride=(1 << 20, 1 << 14, 256),
+                  v_stride=(1 << 20, 1 << 14, 256), dtype=int(rng.choice([rt.PFM_F32, rt.PFM_BF16])))
+        nb = lib.pfm_paged_attention_ws_bytes(c, heads * 2)
+        window, causal = int(rng.integers(1, 16 * width + 1)), int(rng.integers(2))
+        lib.pfm_op_paged_attention(None, c, rows(ts=1 << 14, hs=256), rows(ts=1 << 14, hs=256), heads * 2, 1.0, causal,
+                                   window, P16, nb)
+        assert b"workspace" not in lib.pfm_last_error(), (width, n, heads, b, window, causal)
+
+
+@pytest.mark.parametrize("kw", [dict(k_stride=(4096, 64, 64)), dict(v_stride=(2048, 64, 64)), dict(k_stride=(64, 128, 64)),
+                                dict(k_stride=(1984, 128, 64))], ids=str)
+def test_append_to_interleaved_pages_refused(kw):
+    """strides that step over a head, but on the place of another slot, page or head"""
+    lib = rt.load_library()
+    assert lib.pfm_op_kv_append(None, cache(**kw), rows(), rows(), rows(), rows(), 4, None, 0, 0, None) == E_ARG
+    assert b"overlap" in lib.pfm_last_error()
+
+
+def test_outputs_on_each_other_refused():
+    lib = rt.load_library()
+    assert lib.pfm_op_kv_append(None, cache(), rows(), rows(), rows(), rows(ts=128), 4, None, 0, 0, None) == E_ARG
+    assert lib.pfm_op_paged_attention(None, cache(), rows(), rows(ts=128), 4, 1.0, 1, 0, P16, 1 << 40) == E_ARG
+    assert b"overlap" in lib.pfm_last_error()
+
+
+def test_calls_past_a_launch_refused():
+    """a grid of 2^32 threads or more"""
+    lib = rt.load_library()
+    big = dict(table_width=1, table_stride=1)
+    for kw in (dict(batch=1 << 25, tokens=1 << 25, cu_q=None), dict(batch=1, tokens=(1 << 24) + 1)):
+        c = cache(**big, **kw)
+        assert lib.pfm_op_kv_append(None, c, rows(), rows(), rows(), rows(), 4, None, 0, 0, None) == E_ARG
+        assert lib.pfm_op_paged_attention(None, c, rows(), rows(), 4, 1.0, 1, 0, P16, 1 << 60) == E_ARG
+    c = cache(**big, batch=1 << 20, tokens=1 << 20, cu_q=None, heads=64, k_stride=(1 << 16, 1 << 12, 64),
+              v_stride=(1 << 16, 1 << 12, 64))
+    assert lib.pfm_op_paged_attention(None, c, rows(ts=1 << 13), rows(ts=1 << 13), 64, 1.0, 1, 0, P16, 1 << 60) == E_ARG
+    assert b"one call" in lib.pfm_last_error()
+    assert lib.pfm_op_sample(None, rt.PFM_F32, P16, 20000, (1 << 20) + 1, 20000, P16, None, None, None, None, P16, None,
+                             P16, 1 << 60) == E_ARG
+    assert b"2^20" in lib.pfm_last_error()
+
+
 def test_empty_batches_are_nothing():
     lib = rt.load_library()
     c = cache(batch=0, tokens=0)
