@@ -443,7 +443,7 @@ __device__ __forceinline__ bool is_greedy(const SampleArgs& a, int b) {
 }
 __device__ __forceinline__ Setting setting(const SampleArgs& a, int b, float top) {
     Setting g;
-    const double T = a.temperature ? fmax((double)a.temperature[b], 1e-30) : 1.0;   // the bins' steps stay finite
+    const double T = a.temperature ? fmin(fmax((double)a.temperature[b], 1e-30), 1e30) : 1.0;   // the bins' steps stay finite
     g.greedy = is_greedy(a, b);
     g.r = Row{top, EXPS * 1.4426950408889634074 / T, (float)(2.0 * BINS / (SPAN * T))};
     g.u = a.u[b];

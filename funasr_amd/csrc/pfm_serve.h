@@ -75,11 +75,11 @@ struct PagedKv {
         const int n = kv_len[b];
         return n < 0 ? 0 : n > cap ? (int)cap : n;
     }
-    // New rows [first, end) of sequence b, kept inside [0, tokens).
+    // New rows [first, end) of sequence b, kept inside [0, tokens); none if they descend.
     __device__ __forceinline__ void rows(int b, int& first, int& end) const {
         if (!cu_q) { first = b; end = b + 1; return; }
         first = max(cu_q[b], 0);
-        end = min(cu_q[b + 1], tokens);
+        end = max(min(cu_q[b + 1], tokens), 0);       // end - first stays in 32 bits
     }
 };
 struct Rows {                           // [tokens][heads][dim] with any token / head stride

@@ -51,8 +51,9 @@ int check_cache(const char* fn, const pfm_paged_kv* c, PagedKv& o) {
     if (c->page_size < 1 || c->heads < 1 || c->heads > 65535) return fail(fn, PFM_E_ARG, "page_size and heads must be at least 1, heads at most 65535");
     if (c->head_dim < 8 || c->head_dim > 256 || c->head_dim % 8)
         return fail(fn, PFM_E_ARG, "head_dim must be a multiple of 8 up to 256");
-    if ((long long)c->table_width * c->page_size > 0x7fffff00ll)
-        return fail(fn, PFM_E_ARG, "table_width * page_size must stay under 2^31");
+    // (a position is at least -tokens; less a window it stays in 32 bits)
+    if ((long long)c->table_width * c->page_size > (1ll << 31) - (1 << 25))
+        return fail(fn, PFM_E_ARG, "table_width * page_size must not pass 2^31 - 2^25");
     if (!c->cu_q && c->tokens != c->batch)
         return fail(fn, PFM_E_ARG, "without cu_q every sequence has one new token: tokens must equal batch");
     if (c->batch > 0 && c->tokens > 0) {
@@ -202,7 +203,7 @@ int pfm_op_paged_attention(void* stream, const pfm_paged_kv* cache, const pfm_ro
         a.scale_log2 = scale == 0.f ? 1.f : fabsf(scale) * 1.44269504088896340736f;
         a.q_sign = (scale > 0.f) - (scale < 0.f);
         a.causal = causal ? 1 : 0;
-        a.window = window;
+        a.window = window < (long long)a.c.width * a.c.page + a.c.tokens ? window : 0;     // reaches over all there is
         pfm_paged_attention_plan(cache->dtype, a);
         // a launch has under 2^32 threads
         if ((a.rows_tiles + 2 * a.tiles) * cache->heads >= 1ll << 24)

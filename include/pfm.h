@@ -478,7 +478,7 @@ int pfm_op_ctc_beam(void* stream, const float* am, int L, const float* x, int T,
  *    the strides of page, slot and head in elements; head_dim is contiguous, pointers are aligned to 16 bytes and
  *    strides are multiples of 16 bytes.
  *  - A table entry outside [0, pages) names no page: appends to it are dropped, its keys are not seen. kv_len is cut to
- *    [0, table_width * page_size]. Entries behind the last position are not read.
+ *    [0, table_width * page_size], which must not pass 2^31 - 2^25. Entries behind the last position are not read.
  *  - Rows of q / k / v at or behind cu_q[batch] belong to no sequence: their outputs are left as they were.
  *  - Sequences may share pages that are only read. A page that is appended to belongs to one sequence: what two tokens
  *    appended to one slot in the same call leave there is unspecified. */
@@ -492,7 +492,7 @@ typedef struct pfm_paged_kv {
     const int32_t* kv_len;        /* [batch] */
     const int32_t* cu_q;          /* [batch + 1], ascending from 0, or NULL */
     int32_t dtype, table_width, page_size, heads, head_dim /* multiple of 8, at most 256 */, batch,
-        tokens /* rows of q / k / v */;
+        tokens /* rows of q / k / v; batch and tokens at most 2^24 */;
 } pfm_paged_kv;
 
 /* Rows [tokens][heads][head_dim] at any token and head stride (elements), e.g. a slice of a fused q|k|v projection. */
@@ -519,10 +519,9 @@ int64_t pfm_paged_attention_ws_bytes(const pfm_paged_kv* cache, int q_heads);
 int pfm_op_paged_attention(void* stream, const pfm_paged_kv* cache, const pfm_rows* q, const pfm_rows* out, int q_heads,
                            float scale, int causal, int window, void* ws, int64_t ws_bytes);
 
-/* Draw one token per row of logits [B][ld] (V <= 2^20 used) from given uniform numbers u [B] f32 in [0, 1). Settings
- * [B] device, NULL = off for every row: temperature f32 (<= 0: the largest logit; under 1e-30
- * as 1e-30), top_k int32 (<= 0: off), top_p f32
- * (>= 1: off), min_p f32 (<= 0: off). p = softmax(logits / temperature); tokens in the order of their logits, ties by
+/* Draw one token per row of logits [B][ld] (B <= 2^20, V <= 2^20 used) from given uniform numbers u [B] f32 in [0, 1). Settings
+ * [B] device, NULL = off for every row: temperature f32 (<= 0 or NaN: the largest logit; otherwise
+ * brought into [1e-30, 1e30]), top_k int32 (<= 0: off), top_p f32 (>= 1 or NaN: off), min_p f32 (<= 0 or NaN: off). p = softmax(logits / temperature); tokens in the order of their logits, ties by
  * index; kept are the first top_k, of these the ones before which less than top_p of their mass lies (the first in any
  * case), of these the ones with p >= min_p max(p).
  *   token [B] int32 out: the first kept index, in the vocabulary's order, whose running sum of p exceeds u times the

@@ -106,7 +106,7 @@ def sample(x, u, temperature=None, top_k=None, top_p=None, min_p=None):
             probs.append(1.0)
             continue
         with np.errstate(invalid="ignore", over="ignore"):
-            p = np.where(row == row.max(), 1.0, np.exp((row - row.max()) / T))
+            p = np.where(row == row.max(), 1.0, np.exp((row - row.max()) / min(T, 1e30)))
         order = np.argsort(-row, kind="stable")
         order = order[p[order] > 0]
         if k > 0:

@@ -237,6 +237,30 @@ def test_attend_empty_rows_and_absent_pages(dev):
 
 
 @pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attend_more_new_rows_than_keys(dev, dt, causal):
+    """positions before the first key, under the longest window"""
+    B = Batch([40, 3, 9], [7, 1, 0], D=64, dt=dt)
+    for window in (2 ** 31 - 1, 2 ** 30, 3, 0):
+        attend_check(B, dev, causal=causal, window=window)
+
+
+def test_rows_that_descend_are_none(dev):
+    """cu_q that goes back: the sequence has no rows, whatever the difference is"""
+    B = Batch([2, 3], [5, 6], D=64)
+    kp, vp, table, kv_len, _ = B.on(dev)
+    cu = torch.tensor([4, -2 ** 31, 3], dtype=torch.int32)      # none, then rows 0 .. 2
+    out = torch.full_like(B.q, 7.0)
+    got = rt.op_paged_attention(B.q.to(dev), kp, vp, table, kv_len, cu.to(dev), out=out.to(dev))
+    want, bound, spread = ref.attend(B.q, B.kp, B.vp, B.table, B.kv_len, cu, out=out)
+    check_attend(got.cpu()[:3], want[:3], bound[:3], spread[:3], B, 64)
+    assert (got[3:] == 7).all()
+    rt.op_kv_append(B.k.to(dev), B.v.to(dev), kp, vp, table, kv_len, cu.to(dev))
+    _, wk, wv = ref.append(B.k, B.v, B.kp, B.vp, B.table, B.kv_len, cu)
+    assert torch.equal(kp.cpu().double(), wk) and torch.equal(vp.cpu().double(), wv)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
 def test_attend_rows_behind_the_last_sequence(dev, dt):
     for new, kv in (([5, 3], [50, 20]), ([1, 1], [3000, 2000])):    # unsplit and split keys
         B = Batch(new, kv, D=64, dt=dt)
@@ -464,6 +488,23 @@ def test_sample_settings_out_of_range(dev):
     for u in (1.0, 1.5, math.inf):
         assert rt.op_sample(x.to(dev), full(u).to(dev))[0].tolist() == ref.sample(x, full(min(u, 1.0)))[0]
     assert torch.equal(rt.op_sample(x.to(dev), full(math.nan).to(dev))[0], rt.op_sample(x.to(dev), full(0.0).to(dev))[0])
+
+
+@pytest.mark.parametrize("V", [50, 8404, 20000])
+@pytest.mark.parametrize("T", [math.inf, 1e30, 1e4])
+def test_sample_high_temperatures(dev, V, T):
+    """all logits above -inf alike; the order of tokens is still that of their logits"""
+    B = 12
+    g = torch.Generator().manual_seed(int(V))
+    x = torch.randn(B, V, generator=g) * 5
+    x[1, ::3], x[2, :V // 2], x[3] = -math.inf, -math.inf, 1.0
+    u = torch.rand(B, generator=g)
+    t = torch.full((B,), T)
+    k, p = torch.tensor([0, V // 3 + 1, 2] * 4, dtype=torch.int32), torch.tensor([0.9, 0.5, 1.0, 0.01] * 3)
+    sample_check(dev, x, u, temperature=t)
+    sample_check(dev, x, u, temperature=t, top_p=p)
+    sample_check(dev, x, u, temperature=t, top_k=k)
+    sample_check(dev, x, u, temperature=t, top_k=k, top_p=p)
 
 
 def test_sample_does_not_depend_on_the_batch(dev):

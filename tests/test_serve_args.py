@@ -39,7 +39,8 @@ BAD_CACHE = [dict(dtype=2), dict(dtype=9), dict(batch=-1), dict(tokens=-1), dict
              dict(page_size=0), dict(heads=0), dict(heads=70000), dict(head_dim=0), dict(head_dim=60), dict(head_dim=264),
              dict(k=None), dict(v=None), dict(block_table=None), dict(kv_len=None), dict(cu_q=None), dict(table_stride=2),
              dict(k=P16 + 8), dict(v=P16 + 2), dict(k_stride=(2048, 128, 60)), dict(v_stride=(2044, 128, 64)),
-             dict(k_stride=(-2048, 128, 64)), dict(page_size=1 << 30, table_width=3)]
+             dict(k_stride=(-2048, 128, 64)), dict(page_size=1 << 30, table_width=3),
+             dict(page_size=(1 << 31) - 4096, table_width=1, k_stride=(1 << 38, 128, 64), v_stride=(1 << 38, 128, 64))]
 
 
 @pytest.mark.parametrize("kw", BAD_CACHE, ids=str)
