@@ -275,6 +275,41 @@ __device__ __forceinline__ bool find_tile(const PagedKv& c, int group, int rows,
     return false;
 }
 
+// The same with the sequences of most keys first (among 64 neighbours in the batch), and of each the tiles that see most:
+// a tile runs as long as its keys are many, and long ones that start last leave most of the chip idle at the end. 8
+// sequences of 136 .. 700 new tokens over 1218 .. 6418 keys: 331 us in the batch's order, 279 in this one.
+__device__ __forceinline__ bool find_longest(const PagedKv& c, int group, int rows, int over, int x, int lane, int& b,
+                                             int& tile) {
+    for (int i0 = 0; i0 < c.batch; i0 += 64) {
+        const int i = i0 + lane;
+        int tiles = 0, len = -1;
+        if (i < c.batch) {
+            int first, end;
+            c.rows(i, first, end);
+            const int n = max(end - first, 0) * group;
+            tiles = n > over ? (n + rows - 1) / rows : 0;
+            len = c.len(i);
+        }
+        int all = tiles;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) all += __shfl_xor(all, o, 64);
+        all = __builtin_amdgcn_readfirstlane(all);
+        if (x < all) {
+            int start = 0;                       // tiles of the sequences before the lane's
+            for (int k = 0; k < min(64, c.batch - i0); ++k) {
+                const int n = __builtin_amdgcn_readlane(tiles, k), l = __builtin_amdgcn_readlane(len, k);
+                start += l > len || (l == len && k < lane) ? n : 0;
+            }
+            const int l = __ffsll((long long)__ballot(start <= x && x < start + tiles)) - 1;
+            b = i0 + l;
+            tile = __builtin_amdgcn_readlane(start + tiles, l) - 1 - x;
+            return true;
+        }
+        x -= all;
+    }
+    return false;
+}
+
 // One workgroup = 16 query rows of one sequence and kv head; its waves take key blocks in turn, each with its own V
 // block in LDS and no barrier until the waves' results are joined.
 template <typename T, int DP, int NTILES>
@@ -626,7 +661,7 @@ __global__ __launch_bounds__((TileGeom<T, DP>::NW * 64), 2) void paged_tile_kern
     const int tid = threadIdx.x, lane = tid & 63, wid = uniform(tid >> 6), fr = lane & 31, h = lane >> 5;
     const int hk = blockIdx.x % c.heads;
     int b, tile;
-    if (!find_tile(c, a.group, G::ROWS, a.rows_upto, 0x7fffffff, (gridDim.x - 1 - blockIdx.x) / c.heads, lane, b, tile)) return;
+    if (!find_longest(c, a.group, G::ROWS, a.rows_upto, blockIdx.x / c.heads, lane, b, tile)) return;
     b = uniform(b);
     tile = uniform(tile);
     int first, end;
