@@ -310,6 +310,27 @@ __device__ __forceinline__ bool find_longest(const PagedKv& c, int group, int ro
     return false;
 }
 
+// The keys that the query rows row0 .. row1 of a sequence see, [lo, hi) of all, and their blocks of kb keys.
+struct Span { int pmin, pmax, lo, hi, blk0, nblk; };
+__device__ __forceinline__ Span span_of(const PagedAttnArgs& a, int nq, int len, int row0, int row1, int kb) {
+    Span s;
+    s.pmin = len - nq + a.by_group.div(row0);
+    s.pmax = len - nq + a.by_group.div(row1);
+    s.hi = a.causal ? min(len, s.pmax + 1) : len;
+    s.lo = a.window ? max(0, s.pmin - a.window + 1) : 0;
+    s.blk0 = s.lo / kb;
+    s.nblk = s.hi > s.lo ? (s.hi + kb - 1) / kb - s.blk0 : 0;
+    return s;
+}
+// Parts that a row tile of the rows kernel is split into: enough to fill the chip with parts of at least PART_MIN keys, and
+// none longer than PART_MAX where the launch has that many. 255 caches of 1024 keys and one of 65536, 32 heads on 8: 1758
+// us whole, 493 with the long one in 8 parts; 300 caches of 8192: 1709 us whole, 1742 in halves.
+constexpr int PART_MIN = 256, PART_MAX = 8192;
+__device__ __forceinline__ int parts_of(const PagedAttnArgs& a, int nblk, int kb) {
+    const int keys = nblk * kb, n = max((keys + PART_MAX - 1) / PART_MAX, min(a.fill, (keys + PART_MIN - 1) / PART_MIN));
+    return max(1, min(n, a.splits));
+}
+
 // One workgroup = 16 query rows of one sequence and kv head; its waves take key blocks in turn, each with its own V
 // block in LDS and no barrier until the waves' results are joined.
 template <typename T, int DP, int NTILES>
@@ -338,13 +359,11 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
     const int place = a.by_group.div(row);
     const int head = hk * a.group + row - place * a.group;
     const int pos = len - nq + place;
-    // keys the tile's rows see, as [lo, hi) of all and whether every row sees a whole block
-    const int pmin = len - nq + a.by_group.div(tile * 16), pmax = len - nq + a.by_group.div(tile * 16 + rows - 1);
-    const int hi = a.causal ? min(len, pmax + 1) : len;
-    const int lo = a.window ? max(0, pmin - a.window + 1) : 0;
-    const int blk0 = lo / KB, nblk = hi > lo ? (hi + KB - 1) / KB - blk0 : 0;
-    const int split = blockIdx.y;
-    const int s0 = (int)((long long)nblk * split / a.splits), s1 = (int)((long long)nblk * (split + 1) / a.splits);
+    const Span span = span_of(a, nq, len, tile * 16, tile * 16 + rows - 1, KB);
+    const int pmin = span.pmin, pmax = span.pmax, lo = span.lo, hi = span.hi, blk0 = span.blk0, nblk = span.nblk;
+    const int split = blockIdx.y, parts = uniform(parts_of(a, nblk, KB));
+    if (split >= parts) return;
+    const int s0 = (int)((long long)nblk * split / parts), s1 = (int)((long long)nblk * (split + 1) / parts);
 
     unsigned char* Vs = smem + wid * G::WAVE;
 
@@ -583,7 +602,7 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
         const float mu = mr == -INFINITY ? 0.f : mr;
 #pragma unroll
         for (int w = 0; w < DEC_W; ++w) lsum += ml[w][rr][1] * __builtin_amdgcn_exp2f(ml[w][rr][0] - mu);
-        if (a.splits == 1) {
+        if (parts == 1) {
             const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
             Vec8<T> y;
 #pragma unroll
@@ -1017,12 +1036,19 @@ __global__ __launch_bounds__((TileGeom<T, DP>::NW * 64), 2) void paged_tile_kern
     }
 }
 
+// The parts of a row tile: as the rows kernel takes them (blocks of kb keys), or all `splits` of the tile kernel (kb 0).
+__device__ __forceinline__ int parts_in(const PagedAttnArgs& a, int b, int tile, int per, int nq, int splits, int kb) {
+    if (!kb) return splits;
+    const int row0 = tile * per, row1 = min(row0 + per, nq * a.group) - 1;
+    return uniform(parts_of(a, span_of(a, nq, a.c.len(b), row0, row1, kb).nblk, kb));
+}
+
 // The same for rows of few splits, several rows to a workgroup: a group of lanes holds a row's dims, 4 a lane, and goes
 // over its splits, each lane with one split's weight.
 constexpr int FEW_SPLITS = 16, JOIN_TURNS = 4;
 __host__ __device__ __forceinline__ int join_lanes(int dim) { return dim <= 64 ? 16 : dim <= 128 ? 32 : 64; }
 template <typename T>
-__global__ __launch_bounds__(256) void paged_join_few_kernel(PagedAttnArgs a, int per, int over, int upto, int splits) {
+__global__ __launch_bounds__(256) void paged_join_few_kernel(PagedAttnArgs a, int per, int over, int upto, int splits, int kb) {
     const PagedKv& c = a.c;
     const int lanes = join_lanes(c.dim), at = threadIdx.x % lanes, groups = 256 / lanes, own = JOIN_TURNS * groups;
     const int parts = (per + own - 1) / own;
@@ -1030,6 +1056,8 @@ __global__ __launch_bounds__(256) void paged_join_few_kernel(PagedAttnArgs a, in
     int b, tile, first, end;
     if (!find_tile(c, a.group, per, over, upto, unit / c.heads, threadIdx.x & 63, b, tile)) return;
     c.rows(b, first, end);
+    splits = parts_in(a, b, tile, per, end - first, splits, kb);
+    if (splits == 1) return;
     const int in0 = blockIdx.x % parts * own, row1 = min(tile * per + min(per, in0 + own), (end - first) * a.group);
     const long long nrow = (long long)c.tokens * a.q_heads;
     const int d0 = at * 4;
@@ -1068,7 +1096,7 @@ __global__ __launch_bounds__(256) void paged_join_few_kernel(PagedAttnArgs a, in
 // Joins the splits of one query row, one workgroup each: the splits' sums scaled to their common maximum, then divided
 // once. Rows are numbered as the kernel that split them did, `per` to a row tile.
 template <typename T>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int per, int over, int upto, int splits) {
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int per, int over, int upto, int splits, int kb) {
     const PagedKv& c = a.c;
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
     const int unit = blockIdx.x / per, hk = unit % c.heads;
@@ -1077,6 +1105,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int pe
     c.rows(b, first, end);
     const int row = tile * per + blockIdx.x % per;
     if (row >= (end - first) * a.group) return;
+    splits = parts_in(a, b, tile, per, end - first, splits, kb);
+    if (splits == 1) return;
     const int place = a.by_group.div(row), n = first + place, head = hk * a.group + row - place * a.group;
     const long long nrow = (long long)c.tokens * a.q_heads, r0 = (long long)n * a.q_heads + head;
 
@@ -1121,12 +1151,12 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int pe
 }
 
 template <typename T> hipError_t run_join(const PagedAttnArgs& a, long long tiles, int per, int over, int upto, int splits,
-                                          hipStream_t st) {
+                                          int kb, hipStream_t st) {
     if (splits <= FEW_SPLITS) {
         const int own = JOIN_TURNS * 256 / join_lanes(a.c.dim);
-        paged_join_few_kernel<T><<<(unsigned)(tiles * a.c.heads * ((per + own - 1) / own)), 256, 0, st>>>(a, per, over, upto, splits);
+        paged_join_few_kernel<T><<<(unsigned)(tiles * a.c.heads * ((per + own - 1) / own)), 256, 0, st>>>(a, per, over, upto, splits, kb);
     } else {
-        paged_join_kernel<T><<<(unsigned)(tiles * a.c.heads * per), 256, 0, st>>>(a, per, over, upto, splits);
+        paged_join_kernel<T><<<(unsigned)(tiles * a.c.heads * per), 256, 0, st>>>(a, per, over, upto, splits, kb);
     }
     PFM_LAUNCH_CHECK();
     return hipSuccess;
@@ -1143,7 +1173,7 @@ template <typename T, int DP, int NTILES> hipError_t run_rows(const PagedAttnArg
     if (a.splits == 1) return hipSuccess;
     const int per = c.cu_q ? 16 : std::min(16, a.group);     // a sequence's rows where they are known
     return run_join<T>(a, c.cu_q ? a.rows_tiles : (long long)c.batch * ((a.group + per - 1) / per), per, 0, a.rows_upto,
-                       a.splits, st);
+                       a.splits, R::KB, st);
 }
 template <typename T, int DP>
 hipError_t run_attention(const PagedAttnArgs& a, hipStream_t st) {
@@ -1168,7 +1198,7 @@ hipError_t run_attention(const PagedAttnArgs& a, hipStream_t st) {
         if ((e = pfm_allow_lds<paged_tile_kernel<T, DP>>(G::LDS)) != hipSuccess) return e;
         paged_tile_kernel<T, DP><<<dim3((unsigned)(a.tiles * c.heads), a.tile_splits), G::NW * 64, G::LDS, st>>>(a);
         PFM_LAUNCH_CHECK();
-        if (a.tile_splits > 1) e = run_join<T>(a, a.tiles, G::ROWS, a.rows_upto, 0x7fffffff, a.tile_splits, st);
+        if (a.tile_splits > 1) e = run_join<T>(a, a.tiles, G::ROWS, a.rows_upto, 0x7fffffff, a.tile_splits, 0, st);
         if (e != hipSuccess) return e;
     }
     return hipSuccess;
@@ -1225,7 +1255,12 @@ void pfm_paged_attention_plan(int dtype, PagedAttnArgs& a) {
     auto seen = [&](int rows) {
         return a.window ? std::min<long long>(max_kv, (long long)a.window + rows + (a.causal ? 0 : rows == 16 ? std::min(a.rows_upto, c.tokens) : c.tokens)) : max_kv;
     };
-    a.splits = parts(a.rows_tiles, seen(16), 2048, 256);
+    a.fill = parts(a.rows_tiles, seen(16), 2048, PART_MIN);
+    a.splits = a.fill;
+    if (a.rows_tiles) {      // for long sequences among short ones; 2^14 workgroups that end at once take 10 us
+        const long long units = a.rows_tiles * c.heads, most = (seen(16) + PART_MAX - 1) / PART_MAX;
+        a.splits = (int)std::max<long long>(a.fill, std::min({most, (1ll << 14) / units, 256ll}));
+    }
     a.short_span = seen(16) <= 128;
     // The tile kernel has one workgroup per CU at a time. Split into n parts, its row tiles take so many turns of the 256
     // CUs, each as long as a part and what a part costs beside its keys; the parts' sums are written and read once more.

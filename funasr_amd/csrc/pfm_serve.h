@@ -108,7 +108,8 @@ struct PagedAttnArgs {
     // the launch (pfm_paged_attention_plan)
     int rows_upto;                      // sequences of at most so many query rows go to the rows kernel
     long long rows_tiles, tiles;        // row tiles of the rows and of the tile kernel at most
-    int splits, tile_splits;            // workgroups that share one row tile's keys
+    int splits, tile_splits;            // workgroups that share one row tile's keys, at most
+    int fill;                           // of `splits`, as many as fill the chip
     bool short_span;                    // a row tile of the rows kernel sees at most 128 keys
     float* part;                        // with splits: [splits][tokens * q_heads] rows of dim sums, then max and sum
     float* part_ml;

@@ -345,6 +345,17 @@ def test_attend_many_sequences(dev, n, mq):
     attend_check(B, dev)
 
 
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("new", [0, 2])
+def test_attend_one_long_among_many_short(dev, dt, new):
+    """parts of the long cache alone; new 0: a token each, without cu_q"""
+    kv = [3 + i % 90 for i in range(270)]
+    kv[131], kv[7], kv[0] = 17000, 8193, 0
+    B = Batch([1] * 270 if not new else [new - i % 2 for i in range(270)], kv, hq=16, hk=8, D=16, dt=dt, one=not new)
+    attend_check(B, dev)
+    attend_check(B, dev, window=9000, causal=bool(new))
+
+
 def test_attend_shared_pages(dev):
     """Sequences that share a prefix's pages; one block table row for all (stride 0)."""
     B = Batch([1, 1, 1], [48, 48, 48], dt=BF16, one=True)
