@@ -1232,9 +1232,15 @@ void pfm_paged_attention_plan(int dtype, PagedAttnArgs& a) {
     const long long rows = (long long)c.tokens * a.group, max_kv = (long long)c.width * c.page;
     const int tile_rows = c.dim > 128 ? 128 : 256;
     a.rows_upto = 16;
-    if (!c.cu_q || (dtype == DT_F32 && c.dim > 128)) {   // group rows each; or: too many registers for the tile kernel
+    // Up to 128 dims the rows kernel takes little work whole: row tiles of 16 are that many more workgroups, and a wave's
+    // chain is shorter. The work is row tiles x keys x dims (of all the table reaches: the workspace does not know a window).
+    // Measured, rows against tile kernel, at 4 10^6 (6 10^6): 12 us and 15 (64 dims), 15 and 17 (128), 31 and 37 (128, f32);
+    // at 16 10^6: 22 and 27 (128), 32 and 61 (128, f32); at 23 10^6: 22 and 19 (64); at 47 10^6: 35 and 26 (128).
+    const long long fine = (rows + 15ll * std::min<long long>(c.batch, rows)) / 16;
+    const bool little = c.dim <= 128 && (double)fine * c.heads * max_kv * c.dim <= 2e7;
+    if (!c.cu_q || little || (dtype == DT_F32 && c.dim > 128)) {   // group rows each; or: too many registers for the tile kernel
         a.rows_upto = 0x7fffffff;
-        a.rows_tiles = c.cu_q ? rows / 16 + c.batch : (long long)c.batch * ((a.group + 15) / 16);
+        a.rows_tiles = c.cu_q ? fine : (long long)c.batch * ((a.group + 15) / 16);
         a.tiles = 0;
     } else {
         a.rows_tiles = c.batch;

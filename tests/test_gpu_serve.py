@@ -72,13 +72,19 @@ def half_step(dt):
 
 
 def attend_check(B, dev, q=None, **kw):
+    """The call as it is, and with a table whose further entries name no page: how far it reaches says which kernels run."""
     q = B.q if q is None else q
     kp, vp, table, kv_len, cu = B.on(dev)
-    got = rt.op_paged_attention(q.to(dev), kp, vp, table, kv_len, cu, **kw)
-    torch.cuda.synchronize()
-    want, bound, spread = ref.attend(q, B.kp, B.vp, B.table, B.kv_len, B.cu, **kw)
-    check_attend(got.cpu(), want, bound, spread, B, q.shape[-1])
-    return got
+    (n, hq, D), (_, page, hk) = q.shape, B.kp.shape[:3]
+    far = 2 * 10 ** 7 // ((n * hq // hk // 16 + 1) * hk * D * page) + 1
+    for wide in [torch.full((len(B.kv), 0), -1, dtype=torch.int32), torch.full((len(B.kv), far), -1, dtype=torch.int32)]:
+        got = rt.op_paged_attention(q.to(dev), kp, vp, torch.cat([table, wide.to(dev)], 1), kv_len, cu, **kw)
+        torch.cuda.synchronize()
+        want, bound, spread = ref.attend(q, B.kp, B.vp, torch.cat([B.table, wide], 1), B.kv_len, B.cu, **kw)
+        check_attend(got.cpu(), want, bound, spread, B, D)
+        if not len(wide[0]):
+            first = got
+    return first
 
 
 def check_attend(got, want, bound, spread, B, D):
@@ -216,10 +222,13 @@ def test_attend_one_sequence_in_a_padded_call(dev, dt, used, total):
     q = torch.randn(total, 4, 64).to(dt)
     kp, vp, table, kv_len, cu = B.on(dev)
     out = torch.full((total, 4, 64), 5.0, dtype=dt, device=dev)
-    rt.op_paged_attention(q.to(dev), kp, vp, table, kv_len, cu, out=out)
     want, bound, spread = ref.attend(q, B.kp, B.vp, B.table, B.kv_len, B.cu, out=torch.full((total, 4, 64), 5.0))
-    assert (out[used:] == 5).all()
-    check_attend(out.cpu(), want, bound, spread, B, 64)
+    for more in (0, 20000):
+        out.fill_(5)
+        wide = torch.cat([table, torch.full((1, more), -1, dtype=torch.int32, device=dev)], 1)
+        rt.op_paged_attention(q.to(dev), kp, vp, wide, kv_len, cu, out=out)
+        assert (out[used:] == 5).all()
+        check_attend(out.cpu(), want, bound, spread, B, 64)
 
 
 def test_attend_empty_rows_and_absent_pages(dev):
