@@ -47,55 +47,40 @@ template <typename T> __device__ __forceinline__ void store8(char* p, const Vec8
 }
 
 // ---- append -------------------------------------------------------------------------------------------------------
-// One workgroup per TB tokens. The angles pos * inv_freq are reduced to a turn in 64 bits (a far position's angle has
-// lost its fraction in 32), the sine and cosine are taken once per token and pair and shared by all heads through LDS.
+// (x1, x2) -> (x1 cos - x2 sin, x2 cos + x1 sin) by the angle pos * inv_freq, then one rounding to the type. It is a copy
+// that memory bounds: one workgroup per token (four tokens each: 95 us where this takes 88, 16384 tokens of 32 query and 8
+// kv heads of 128 dims in 16 bits). The angles are reduced to a turn in 64 bits (a far position's angle has lost its
+// fraction in 32), the sine and cosine are taken once per pair and shared by all heads through LDS; a thread moves 16 or
+// 32 bytes of a head at a time. One token of 64 sequences takes 4 us: three reads that wait for each other, and a launch.
 constexpr int AP_T = 256;
 
-template <typename T, int TB>
+template <typename T>
 __global__ __launch_bounds__(AP_T) void kv_append_kernel(AppendArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    __shared__ int dst_page[TB];
-    __shared__ int dst_slot[TB];            // -1: the row has no sequence; -2: rotated, but no place to write
-    __shared__ int turn_pos[TB];
-    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, n = blockIdx.x;
     const int half = a.inv_freq ? a.rot / 2 : 0;
-    float2* cs = (float2*)smem;             // [TB][half] (cos, sin)
+    float2* cs = (float2*)smem;             // [half] (cos, sin)
     const PagedKv& c = a.c;
-    const int n0 = blockIdx.x * TB;
 
-    for (int t = wid; t < TB; t += AP_T / 64) {
-        const int n = n0 + t;
-        int slot = -1, pos = 0;
-        int page = 0;
-        if (n < c.tokens) {
-            const int b = seq_of_row(c, n, lane);
-            int first, end;
-            if (b < c.batch) {
-                c.rows(b, first, end);
-                if (n >= first) {
-                    const int len = c.len(b), at = len - (end - first) + (n - first);
-                    slot = -2;
-                    if (at >= 0 && at < len) {
-                        const int pi = c.by_page.div(at);
-                        page = page_of(c, b, pi);
-                        if (page >= 0) slot = at - pi * c.page;
-                    }
-                    pos = a.pos ? a.pos[n] : at;
-                }
-            }
-        }
-        if (lane == 0) { dst_page[t] = page; dst_slot[t] = slot; turn_pos[t] = pos; }
+    const int b = seq_of_row(c, n, lane);   // every wave for itself
+    if (b >= c.batch) return;
+    int first, end;
+    c.rows(b, first, end);
+    if (n < first) return;
+    const int len = c.len(b), at = len - (end - first) + (n - first);
+    int page = -1, slot = 0;                // no page: rotated, but no place to write
+    if (at >= 0 && at < len) {
+        const int pi = c.by_page.div(at);
+        page = page_of(c, b, pi);
+        slot = at - pi * c.page;
     }
-    __syncthreads();
-    for (int i = tid; i < TB * half; i += AP_T) {
-        const int t = i / half, f = i - t * half;
-        if (dst_slot[t] != -1) {
-            double r = (double)turn_pos[t] * (double)a.inv_freq[f] * 0.15915494309189533577;   // turns
-            r -= rint(r);
-            float s, co;
-            sincospif((float)(2.0 * r), &s, &co);
-            cs[i] = make_float2(co, s);
-        }
+    const int pos = a.pos ? a.pos[n] : at;
+    for (int f = tid; f < half; f += AP_T) {
+        double r = (double)pos * (double)a.inv_freq[f] * 0.15915494309189533577;   // turns
+        r -= rint(r);
+        float s, co;
+        sincospif((float)(2.0 * r), &s, &co);
+        cs[f] = make_float2(co, s);
     }
     __syncthreads();
 
@@ -104,11 +89,8 @@ __global__ __launch_bounds__(AP_T) void kv_append_kernel(AppendArgs a) {
     const int turned = (a.q_heads + c.heads) * h8, kept = (a.q_heads + c.heads) * rest8, vals = c.heads * D8;
     const int per = turned + kept + vals;
     constexpr int E = sizeof(T);
-    for (int i = tid; i < TB * per; i += AP_T) {
-        const int t = i / per;
-        int w = i - t * per;
-        const int n = n0 + t, slot = dst_slot[t];
-        if (slot == -1) continue;
+    for (int i = tid; i < per; i += AP_T) {
+        int w = i;
         if (w < turned + kept) {
             const bool turn = w < turned;
             if (!turn) w -= turned;
@@ -123,9 +105,9 @@ __global__ __launch_bounds__(AP_T) void kv_append_kernel(AppendArgs a) {
                 dst = a.qo.p + ((long long)n * a.qo.ts + (long long)h * a.qo.hs) * E;
             } else {
                 h -= a.q_heads;
-                if (slot < 0) continue;
+                if (page < 0) continue;
                 src = a.k.p + ((long long)n * a.k.ts + (long long)h * a.k.hs) * E;
-                dst = c.k_head(h) + c.k_at(dst_page[t], slot);
+                dst = c.k_head(h) + c.k_at(page, slot);
             }
             if (!turn) {
                 const int o = (2 * h8 + j) * 8 * E;
@@ -135,7 +117,7 @@ __global__ __launch_bounds__(AP_T) void kv_append_kernel(AppendArgs a) {
             // the two pieces of a pair group: (x1 | x2) half a rotated width apart, or 16 neighbours
             const int o1 = a.interleaved ? j * 16 * E : j * 8 * E, o2 = a.interleaved ? o1 + 8 * E : o1 + half * E;
             Vec8<T> p = load8<T>(src + o1), q = load8<T>(src + o2), p2, q2;
-            const float2* m = cs + t * half + j * 8;
+            const float2* m = cs + j * 8;
             if (a.interleaved) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -159,9 +141,9 @@ __global__ __launch_bounds__(AP_T) void kv_append_kernel(AppendArgs a) {
             store8<T>(dst + o2, q2);
         } else {
             w -= turned + kept;
-            if (slot < 0) continue;
+            if (page < 0) continue;
             const int h = w / D8, o = (w - h * D8) * 8 * E;
-            store8<T>(c.v_head(h) + c.v_at(dst_page[t], slot) + o,
+            store8<T>(c.v_head(h) + c.v_at(page, slot) + o,
                       load8<T>(a.v.p + ((long long)n * a.v.ts + (long long)h * a.v.hs) * E + o));
         }
     }
@@ -1213,11 +1195,7 @@ hipError_t run_attention(const PagedAttnArgs& a, hipStream_t st) {
 template <typename T>
 hipError_t run_append(const AppendArgs& a, hipStream_t st) {
     const int half = a.inv_freq ? a.rot / 2 : 0;
-    if (a.c.tokens <= 1024) {
-        kv_append_kernel<T, 1><<<a.c.tokens, AP_T, half * sizeof(float2), st>>>(a);
-    } else {
-        kv_append_kernel<T, 4><<<(a.c.tokens + 3) / 4, AP_T, 4 * half * sizeof(float2), st>>>(a);
-    }
+    kv_append_kernel<T><<<a.c.tokens, AP_T, half * sizeof(float2), st>>>(a);
     PFM_LAUNCH_CHECK();
     return hipSuccess;
 }
@@ -1261,7 +1239,10 @@ void pfm_paged_attention_plan(int dtype, PagedAttnArgs& a) {
     auto seen = [&](int rows) {
         return a.window ? std::min<long long>(max_kv, (long long)a.window + rows + (a.causal ? 0 : rows == 16 ? std::min(a.rows_upto, c.tokens) : c.tokens)) : max_kv;
     };
-    a.fill = parts(a.rows_tiles, seen(16), 2048, PART_MIN);
+    // Few caches in many parts: as many workgroups as the chip holds at once. 2 of 131072 keys, 32 heads on 8, 202 us and 217
+    // with twice as many; 8 of up to 32768 167 and 174. Many caches of different lengths: twice as many, for an even
+    // end. 64 of up to 16384 keys 441 and 494 with half as many (of 9216 keys each 435 and 423).
+    a.fill = parts(a.rows_tiles, seen(16), a.rows_tiles * c.heads <= 128 ? 1024 : 2048, PART_MIN);
     a.splits = a.fill;
     if (a.rows_tiles) {      // for long sequences among short ones; 2^14 workgroups that end at once take 10 us
         const long long units = a.rows_tiles * c.heads, most = (seen(16) + PART_MAX - 1) / PART_MAX;
