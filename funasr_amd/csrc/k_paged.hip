@@ -150,6 +150,12 @@ __global__ __launch_bounds__(AP_T) void kv_append_kernel(AppendArgs a) {
 }
 
 // ---- attention ----------------------------------------------------------------------------------------------------
+// o_i = sum_j p_ij v_j / sum_j p_ij with p_ij = exp(scale q_i . k_j - m_i), in one pass over the keys: m is the running
+// maximum, and o and the sum are scaled down when it grows. The exponent's base is 2 (log2 e goes into the scale). All
+// of it is held in 32 bits; p is rounded to the cache's 16-bit type for the second product, relative to itself by half
+// a step, as the values are. Two kernels: rows (16 query rows, memory bounds it: the single tokens) and tile (256 query
+// rows that share their keys, the matrix products bound it: the chunks of prompts), and a join where keys are split.
+//
 // Operand traits. The products run swapped, S^T = K Q^T and O^T = V^T P^T: in both accumulators the query row is the
 // lane (lane & 15), so a row's maximum, sum and rescale are per lane, and the probabilities of two 16-key tiles are, as
 // they stand in S^T's registers, the second product's operand: its contraction index 8 g + j is key 4 g + j of the
@@ -314,7 +320,11 @@ __device__ __forceinline__ int parts_of(const PagedAttnArgs& a, int nblk, int kb
 }
 
 // One workgroup = 16 query rows of one sequence and kv head; its waves take key blocks in turn, each with its own V
-// block in LDS and no barrier until the waves' results are joined.
+// block in LDS and no barrier until the waves' results are joined. The matrix instruction has 16 rows whether the group of
+// query heads fills them or not: its time is hidden. K goes from memory to registers as the product's operand, V over
+// LDS, which transposes it; both of the next block are under way while this one is worked on (387 us without, 265 with).
+// 64 caches of 1000 .. 9216 keys, 32 heads on 8 of 128 dims in 16 bits: 1.20 GB in 254 .. 271 us, 4.4 .. 4.7 TB/s, where a
+// copy of 4 GiB makes 4.75. One cache of 201 keys takes 10 us, of which most is waiting: length, page id, keys, values.
 template <typename T, int DP, int NTILES>
 __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a) {
     using G = DecGeom<T, DP, NTILES>;
@@ -601,6 +611,15 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
 }
 
 // ---- chunks: row tiles that share their keys through LDS
+// 8 waves of 32 query rows (from 129 dims on, two waves share 32 rows, each with half of the dims of V). K and V
+// tiles go from memory straight to LDS, three tiles ahead, in rings of four; a piece's place in its row is
+// exclusive-ored with the row, so that no read meets a bank twice as often as it must. The scores of the next tile are
+// computed under the exponentials of this one, and o is rescaled only where a maximum has grown by more than 2^8: p then
+// stays under 2^8 in 32 bits, and under it in 16 bits too. 2 prompts of 4096 tokens over 8192 and 6125 keys, 32 heads on 8 of
+// 128 dims in 16 bits: 686 GFLOP in 763 .. 794 us, 865 .. 900 TFLOP/s, where a product of 8192^3 makes 1118. The chip lowers
+// its clock to 2.0 GHz under it, and exponentials, maxima and conversions hold the vector units as long as the products
+// hold the matrix units: leaving out any one of them saves its own share alone.
+//
 // The same swapped products on 32 x 32 tiles: a wave owns 32 query rows (row = lane & 31, h = lane >> 5), register e of
 // a score tile is key kappa(e) + 4 h, and registers 8 s .. 8 s + 7 are the probabilities of the second product's s-th
 // 16 keys in the order key 16 s + 4 h + j, 16 s + 8 + 4 h + j - 4.
@@ -1026,7 +1045,8 @@ __device__ __forceinline__ int parts_in(const PagedAttnArgs& a, int b, int tile,
 }
 
 // The same for rows of few splits, several rows to a workgroup: a group of lanes holds a row's dims, 4 a lane, and goes
-// over its splits, each lane with one split's weight.
+// over its splits, each lane with one split's weight. 64 caches of 4096 keys in 4 parts: attention takes 222 us, 253 with a
+// workgroup per row. More parts go to a workgroup per row, whose threads share them (64 parts: 7 us).
 constexpr int FEW_SPLITS = 16, JOIN_TURNS = 4;
 __host__ __device__ __forceinline__ int join_lanes(int dim) { return dim <= 64 ? 16 : dim <= 128 ? 32 : 64; }
 template <typename T>
@@ -1165,9 +1185,9 @@ hipError_t run_attention(const PagedAttnArgs& a, hipStream_t st) {
     const PagedKv& c = a.c;
     hipError_t e = hipSuccess;
     if (a.rows_tiles) {
-        // 32-bit heads: blocks of 32 keys leave a SIMD one wave beyond 64 dims, blocks of 16 two (34 caches of 8230 keys
-        // and 96 dims: 143 -> 88 us); short spans take the longer block all the same (64 streams over 70 keys: 16 us, 19
-        // with 16). Beyond 128 dims it does not fit the registers.
+        // 32-bit heads: blocks of 32 keys leave a SIMD one wave beyond 64 dims, blocks of 16 two (34 caches of 8230 keys,
+        // 8 heads on 2 of 96 dims: 180 us and 127); short spans take the longer block all the same (64
+        // streams' chunks of 15 rows over 70 keys, 4 heads of 128: 16 us, 19 in blocks of 16). Beyond 128 dims it does not fit the registers.
         if constexpr (sizeof(T) == 4 && DP > 64) {
             if (DP > 128 || !a.short_span) e = run_rows<T, DP, 1>(a, st);
             else if constexpr (DP <= 128) e = run_rows<T, DP, 2>(a, st);
@@ -1239,6 +1259,7 @@ void pfm_paged_attention_plan(int dtype, PagedAttnArgs& a) {
     auto seen = [&](int rows) {
         return a.window ? std::min<long long>(max_kv, (long long)a.window + rows + (a.causal ? 0 : rows == 16 ? std::min(a.rows_upto, c.tokens) : c.tokens)) : max_kv;
     };
+    // (parts of 256 keys at least: 32 caches of 1000 keys take 32 us, 36 in parts of 128; 4 of 2048 16 us, 20 in parts of 512)
     // Few caches in many parts: as many workgroups as the chip holds at once. 2 of 131072 keys, 32 heads on 8, 202 us and 217
     // with twice as many; 8 of up to 32768 167 and 174. Many caches of different lengths: twice as many, for an even
     // end. 64 of up to 16384 keys 441 and 494 with half as many (of 9216 keys each 435 and 423).

@@ -146,6 +146,26 @@ static void op_validation() {
     expect_rc(pfm_op_fsmn_bf16(nullptr, nullptr, &i1, f4, f4, 1, 1, 4, 3, 1), PFM_E_ARG, "op_fsmn_bf16 null");
     expect_rc(pfm_op_cif(nullptr, nullptr, f4, f4, f4, tok, tok, 1, 1, 4, 4), PFM_E_ARG, "op_cif null");
     expect_rc(pfm_op_ctc_collapse(nullptr, nullptr, 4, &i1, 1, 0, tok, 4, tok), PFM_E_ARG, "op_ctc_collapse null");
+    {   // decoding over a paged cache
+        pfm_paged_kv kv{};
+        const pfm_rows r{nullptr, 8, 8};
+        expect_rc(pfm_op_kv_append(nullptr, nullptr, &r, &r, &r, &r, 1, nullptr, 0, 0, nullptr), PFM_E_ARG, "kv_append null cache");
+        expect_rc(pfm_op_paged_attention(nullptr, nullptr, &r, &r, 1, 1.f, 1, 0, nullptr, 0), PFM_E_ARG, "paged_attention null cache");
+        kv.dtype = PFM_BF16;
+        kv.table_width = kv.page_size = kv.heads = kv.batch = kv.tokens = 1;
+        kv.head_dim = 8;
+        expect_rc(pfm_op_kv_append(nullptr, &kv, &r, &r, &r, &r, 1, nullptr, 0, 0, nullptr), PFM_E_ARG, "kv_append null pointers");
+        expect_rc(pfm_op_paged_attention(nullptr, &kv, &r, &r, 1, 1.f, 1, 0, nullptr, 0), PFM_E_ARG, "paged_attention null pointers");
+        kv.head_dim = 12;
+        expect_rc(pfm_op_kv_append(nullptr, &kv, nullptr, nullptr, nullptr, nullptr, 0, nullptr, 0, 0, nullptr), PFM_E_ARG, "kv_append head_dim");
+        kv.page_size = 0;
+        expect_rc(pfm_op_paged_attention(nullptr, &kv, nullptr, nullptr, 1, 1.f, 1, 0, nullptr, 0), PFM_E_ARG, "paged_attention page_size");
+        expect(pfm_paged_attention_ws_bytes(nullptr, 1) == 0 && pfm_paged_attention_ws_bytes(&kv, 0) == 0, "paged_attention ws of nothing");
+        expect_rc(pfm_op_sample(nullptr, PFM_F32, nullptr, 4, 1, 4, f4, nullptr, nullptr, nullptr, nullptr, tok, nullptr, nullptr, 0), PFM_E_ARG, "op_sample null");
+        expect_rc(pfm_op_sample(nullptr, 9, f4, 4, 1, 4, f4, nullptr, nullptr, nullptr, nullptr, tok, nullptr, nullptr, 0), PFM_E_ARG, "op_sample dtype");
+        expect_rc(pfm_op_sample(nullptr, PFM_F32, f4, 20000, 2, 20000, f4, nullptr, nullptr, nullptr, nullptr, tok, nullptr, nullptr, 0), PFM_E_ARG, "op_sample workspace");
+        expect(pfm_sample_ws_size(0, 4) == 0 && pfm_sample_ws_size(1, 100) == 0 && pfm_sample_ws_size(1, 100000) > 0, "sample ws");
+    }
     expect_rc(pfm_op_ctc_beam(nullptr, nullptr, 1, f4, 1, &i1, &i1, 1, 4, 4, 0.3f, 0.f, 1, 0, 1, 2, 0, tok, 4, tok, f4),
               PFM_E_ARG, "op_ctc_beam null");
     expect_rc(pfm_op_ctc_beam(nullptr, f4, 1, f4, 1, &i1, &i1, 1, 4, 99, 0.3f, 0.f, 1, 0, 1, 2, 0, tok, 4, tok, f4),
