@@ -915,6 +915,8 @@ def op_paged_attention(q, k_pages, v_pages, block_table, kv_len, cu_q=None, scal
     lib = load_library()
     if q.dim() != 3:
         raise PfmError("q must be [tokens, q_heads, head_dim]")
+    if not 0 <= window < 1 << 31:
+        raise PfmError("window must be in [0, 2^31): 0 for none")
     n, hq, _ = q.shape
     dev, dt = k_pages.device, k_pages.dtype
     kv = _paged_kv(torch, k_pages, v_pages, block_table, kv_len, cu_q, n)

@@ -206,6 +206,13 @@ def test_wrappers_refuse_host_tensors_and_extras():
             call()
 
 
+@pytest.mark.parametrize("window", [-1, 1 << 31, (1 << 32) + 5])
+def test_wrapper_refuses_windows_past_32_bits(window):
+    a = _args()
+    with pytest.raises(rt.PfmError, match="window"):
+        rt.op_paged_attention(a["q"], a["kp"], a["vp"], a["table"], a["kv_len"], window=window)
+
+
 def test_struct_layout_matches_header():
     """ctypes layouts against the C compiler's, by the header's field order and sizes."""
     assert ctypes.sizeof(rt.PfmRows) == 24 and ctypes.sizeof(rt.PfmPagedKv) == 8 * 13 + 4 * 7 + 4
