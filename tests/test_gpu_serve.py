@@ -510,6 +510,15 @@ def test_sample_settings_out_of_range(dev):
     assert torch.equal(rt.op_sample(x.to(dev), full(math.nan).to(dev))[0], rt.op_sample(x.to(dev), full(0.0).to(dev))[0])
 
 
+@pytest.mark.parametrize("V", [12287, 12288, 12289])
+@pytest.mark.parametrize("mode", ["plain", "topp", "mixed"])
+def test_sample_about_the_longest_row_of_one_workgroup(dev, V, mode):
+    B = 9
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(B, V, generator=g) * 3
+    sample_check(dev, x, torch.rand(B, generator=g), **settings(B, mode, V))
+
+
 @pytest.mark.parametrize("V", [50, 8404, 20000])
 @pytest.mark.parametrize("T", [math.inf, 1e30, 1e4])
 def test_sample_high_temperatures(dev, V, T):
