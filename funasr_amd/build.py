@@ -58,7 +58,8 @@ def _stale(obj: str, deps) -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
-def build(verbose: bool = False, jobs: int = 8) -> str:
+def build(verbose: bool = False, jobs: int = 8, force: bool = False) -> str:
+    """The library, of what is older than its sources; force: of everything (an object does not tell its flags)."""
     os.makedirs(OBJ_DIR, exist_ok=True)
     cc = hipcc()
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.hip")))
@@ -68,7 +69,7 @@ def build(verbose: bool = False, jobs: int = 8) -> str:
     for s in srcs:
         o = os.path.join(OBJ_DIR, os.path.basename(s) + ".o")
         objs.append(o)
-        if _stale(o, [s] + hdrs):
+        if force or _stale(o, [s] + hdrs):
             todo.append((s, o))
 
     def compile_one(so):
