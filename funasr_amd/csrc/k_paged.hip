@@ -601,11 +601,12 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
             for (int e = 0; e < 8; ++e) y.x[e] = from_f<T>(lsum == 0.f ? 0.f : x[e] * inv);
             store8<T>(a.o.p + ((long long)n * a.o.ts + (long long)hd * a.o.hs) * E + d0 * E, y);
         } else {
-            const long long pr = (long long)split * c.tokens * a.q_heads + (long long)n * a.q_heads + hd;
-            float* dst = a.part + pr * c.dim + d0;
+            const PagedParts& w = a.rows_part;
+            const long long pr = split * w.rows + (w.by_tile ? blockIdx.x * 16ll + rr : (long long)n * a.q_heads + hd);
+            float *dst = a.ws + pr * c.dim + d0, *dst_ml = a.ws + a.splits * w.rows * c.dim + 2 * pr;
             *(f32x4*)dst = f32x4{x[0], x[1], x[2], x[3]};
             *(f32x4*)(dst + 4) = f32x4{x[4], x[5], x[6], x[7]};
-            if (d0 == 0) { a.part_ml[2 * pr] = mr; a.part_ml[2 * pr + 1] = lsum; }
+            if (d0 == 0) { dst_ml[0] = mr; dst_ml[1] = lsum; }
         }
     }
 }
@@ -1024,8 +1025,8 @@ __global__ __launch_bounds__((TileGeom<T, DP>::NW * 64), 2) void paged_tile_kern
                 else *(float2*)(dst + dd * E) = *(const float2*)y;
             }
     } else {
-        const long long pr = (long long)split * c.tokens * a.q_heads + (long long)n * a.q_heads + head;
-        float* dst = a.part + pr * c.dim;
+        const long long pr = split * a.tile_part.rows + (long long)n * a.q_heads + head;
+        float *dst = a.ws + pr * c.dim, *dst_ml = a.ws + a.tile_splits * a.tile_part.rows * c.dim + 2 * pr;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -1033,7 +1034,7 @@ __global__ __launch_bounds__((TileGeom<T, DP>::NW * 64), 2) void paged_tile_kern
                 const int dd = dim0 + 32 * d + kappa(e) + 4 * h;
                 if (dd < c.dim) *(f32x4*)(dst + dd) = f32x4{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
             }
-        if (h == 0 && dim0 == 0) { a.part_ml[2 * pr] = m; a.part_ml[2 * pr + 1] = l; }
+        if (h == 0 && dim0 == 0) { dst_ml[0] = m; dst_ml[1] = l; }
     }
 }
 
@@ -1042,6 +1043,17 @@ __device__ __forceinline__ int parts_in(const PagedAttnArgs& a, int b, int tile,
     if (!kb) return splits;
     const int row0 = tile * per, row1 = min(row0 + per, nq * a.group) - 1;
     return uniform(parts_of(a, span_of(a, nq, a.c.len(b), row0, row1, kb).nblk, kb));
+}
+
+// The parts that the join reads: sums of split 0's first row, maxima and sums, rows of a split.
+struct PartsIn {
+    const float *sum, *ml;
+    long long rows;
+    bool by_tile;
+};
+__device__ __forceinline__ PartsIn parts_at(const PagedAttnArgs& a, int kb) {
+    const PagedParts& w = kb ? a.rows_part : a.tile_part;
+    return PartsIn{a.ws, a.ws + (kb ? a.splits : a.tile_splits) * w.rows * a.c.dim, w.rows, w.by_tile};
 }
 
 // The same for rows of few splits, several rows to a workgroup: a group of lanes holds a row's dims, 4 a lane, and goes
@@ -1061,19 +1073,19 @@ __global__ __launch_bounds__(256) void paged_join_few_kernel(PagedAttnArgs a, in
     splits = parts_in(a, b, tile, per, end - first, splits, kb);
     if (splits == 1) return;
     const int in0 = blockIdx.x % parts * own, row1 = min(tile * per + min(per, in0 + own), (end - first) * a.group);
-    const long long nrow = (long long)c.tokens * a.q_heads;
+    const PartsIn in = parts_at(a, kb);
     const int d0 = at * 4;
     for (int row = tile * per + in0 + threadIdx.x / lanes; row < row1; row += groups) {
         const int place = a.by_group.div(row), n = first + place, head = hk * a.group + row - place * a.group;
-        const long long r0 = (long long)n * a.q_heads + head;
+        const long long r0 = in.by_tile ? unit * 16ll + row - tile * per : (long long)n * a.q_heads + head;
         f32x4 x[FEW_SPLITS];
 #pragma unroll
         for (int s = 0; s < FEW_SPLITS; ++s) {
             x[s] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (s < splits && d0 < c.dim) x[s] = *(const f32x4*)(a.part + (s * nrow + r0) * c.dim + d0);
+            if (s < splits && d0 < c.dim) x[s] = *(const f32x4*)(in.sum + (s * in.rows + r0) * c.dim + d0);
         }
         float2 ml = make_float2(-INFINITY, 0.f);
-        if (at < splits) ml = *(const float2*)(a.part_ml + 2 * (at * nrow + r0));
+        if (at < splits) ml = *(const float2*)(in.ml + 2 * (at * in.rows + r0));
         float m = ml.x;
         for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 16));
         m = __shfl(m, 0, lanes);
@@ -1110,14 +1122,15 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int pe
     splits = parts_in(a, b, tile, per, end - first, splits, kb);
     if (splits == 1) return;
     const int place = a.by_group.div(row), n = first + place, head = hk * a.group + row - place * a.group;
-    const long long nrow = (long long)c.tokens * a.q_heads, r0 = (long long)n * a.q_heads + head;
+    const PartsIn in = parts_at(a, kb);
+    const long long r0 = in.by_tile ? unit * 16ll + row - tile * per : (long long)n * a.q_heads + head;
 
     // the splits' weights (at most one per thread)
     __shared__ float ws[256], ms[4], ls[4];
     __shared__ f32x4 xs[4][64];
     const int t = threadIdx.x;
     float2 ml = make_float2(-INFINITY, 0.f);
-    if (t < splits) ml = *(const float2*)(a.part_ml + 2 * (t * nrow + r0));
+    if (t < splits) ml = *(const float2*)(in.ml + 2 * (t * in.rows + r0));
     const float mw = wave_max(ml.x);
     if (lane == 0) ms[wid] = mw;
     __syncthreads();
@@ -1133,7 +1146,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int pe
     f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
     for (int s = wid * (64 / lanes) + sub; s < splits; s += step)
-        if (d0 < c.dim) x += *(const f32x4*)(a.part + (s * nrow + r0) * c.dim + d0) * ws[s];
+        if (d0 < c.dim) x += *(const f32x4*)(in.sum + (s * in.rows + r0) * c.dim + d0) * ws[s];
     for (int o = lanes; o < 64; o <<= 1) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] += __shfl_xor(x[e], o, 64);
@@ -1299,6 +1312,11 @@ void pfm_paged_attention_plan(int dtype, PagedAttnArgs& a) {
         a.tile_splits = best_of(max_kv, a.tiles * c.heads < 65536 ? 64 : 1);
         if (a.window) a.tile_splits = best_of(seen(tile_rows), a.tile_splits);     // the workspace is that of no window
     }
+    // The rows kernel takes few of a call's rows where the tile kernel is there too: numbered by its row tiles they need
+    // no more than 16 places for each sequence and kv head.
+    a.tile_part = {(long long)c.tokens * a.q_heads, false};
+    a.rows_part = a.tile_part;
+    if (c.cu_q && a.rows_tiles * c.heads * 16 < a.rows_part.rows) a.rows_part = {a.rows_tiles * c.heads * 16, true};
 }
 hipError_t pfm_paged_attention(int dtype, const PagedAttnArgs& a, hipStream_t st) {
     if (dtype == DT_F32) return run_attention<float>(a, st);

@@ -97,6 +97,13 @@ struct AppendArgs {
 };
 hipError_t pfm_kv_append(int dtype, const AppendArgs& a, hipStream_t st);
 
+// Where a kernel whose row tiles are split leaves its parts in the workspace: [splits][rows] sums of dim floats, then
+// as many pairs of maximum and sum. A query row's place is token * q_heads + head, or that of its row tile (by_tile).
+struct PagedParts {
+    long long rows;
+    bool by_tile;
+};
+
 struct PagedAttnArgs {
     PagedKv c;
     Rows q, o;
@@ -111,8 +118,8 @@ struct PagedAttnArgs {
     int splits, tile_splits;            // workgroups that share one row tile's keys, at most
     int fill;                           // of `splits`, as many as fill the chip
     bool short_span;                    // a row tile of the rows kernel sees at most 128 keys
-    float* part;                        // with splits: [splits][tokens * q_heads] rows of dim sums, then max and sum
-    float* part_ml;
+    PagedParts rows_part, tile_part;
+    float* ws;                          // the parts of one kernel after the other's
 };
 void pfm_paged_attention_plan(int dtype, PagedAttnArgs& a);   // of a.c, a.q_heads, a.group and a.window
 hipError_t pfm_paged_attention(int dtype, const PagedAttnArgs& a, hipStream_t st);

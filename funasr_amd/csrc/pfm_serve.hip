@@ -122,8 +122,8 @@ int hip(const char* fn, hipError_t e) { return e == hipSuccess ? PFM_OK : fail(f
     } while (0)
 
 long long attention_ws(const PagedAttnArgs& a) {
-    const int s = std::max(a.splits, a.tile_splits);
-    return s > 1 ? s * (long long)a.c.tokens * a.q_heads * (a.c.dim + 2) * 4 : 0;
+    const long long rows = std::max(a.splits > 1 ? a.splits * a.rows_part.rows : 0, a.tile_splits > 1 ? a.tile_splits * a.tile_part.rows : 0);
+    return rows * (a.c.dim + 2) * 4;
 }
 
 }  // namespace
@@ -211,13 +211,10 @@ int pfm_op_paged_attention(void* stream, const pfm_paged_kv* cache, const pfm_ro
         const long long need = attention_ws(a);
         if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
             return fail(fn, PFM_E_ARG, "workspace missing, not aligned to 16 bytes or under pfm_paged_attention_ws_bytes");
-        if (need) {
-            a.part = (float*)ws;
-            a.part_ml = a.part + (long long)std::max(a.splits, a.tile_splits) * cache->tokens * q_heads * cache->head_dim;
-        }
+        if (need) a.ws = (float*)ws;
         const PfmDevOp ops[] = {{"q", a.q.p}, {"out", a.o.p}, {"k_pages", a.c.k}, {"v_pages", a.c.v},
                                 {"block_table", a.c.table}, {"kv_len", a.c.kv_len}, {"cu_q", a.c.cu_q},
-                                {"ws", a.part}};
+                                {"ws", a.ws}};
         TRY(pfm_check_dev_ops(fn, ops, (int)(sizeof(ops) / sizeof(ops[0]))));
         return hip(fn, pfm_paged_attention(cache->dtype, a, (hipStream_t)stream));
     });

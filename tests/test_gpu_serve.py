@@ -333,6 +333,19 @@ def test_attend_long_and_split(dev, dt):
     attend_check(Batch([2, 1], [9000, 40], hq=2, hk=1, D=64, page=16, dt=dt, seed=3), dev, window=300)
 
 
+@pytest.mark.parametrize("dt,D", [(F32, 64), (BF16, 128), (F16, 256)])
+@pytest.mark.parametrize("far", [9000, 4000])
+def test_attend_few_rows_over_long_caches_among_prompts(dev, dt, D, far):
+    """Both kernels in one call, the few rows' keys split (into more and into fewer parts than 16): their parts in the
+    workspace are numbered by row tiles. Sequences without rows and with more than one head group per tile among them."""
+    B = Batch([1, 60, 0, 2, 3, 90], [far, 77, 500, far // 2, 130, 300], hq=8, hk=2, D=D, page=16, dt=dt, seed=far)
+    lib, (kp, vp, table, kv_len, cu) = rt.load_library(), B.on(dev)
+    kv = rt._paged_kv(torch, kp, vp, table, kv_len, cu, 156)
+    assert lib.pfm_paged_attention_ws_bytes(kv, 8) > 0
+    attend_check(B, dev)
+    attend_check(B, dev, window=far // 2 + 9, causal=False)
+
+
 def test_attend_large_scores(dev):
     """Scores of thousands: one key takes all; the running maximum rises late."""
     B = Batch([1, 30], [200, 400], hq=2, hk=2, D=64, dt=F32, seed=3)

@@ -121,6 +121,21 @@ def test_window_takes_the_workspace_of_no_window():
         assert b"workspace" not in lib.pfm_last_error(), (width, n, heads, b, window, causal)
 
 
+def ws_bytes(batch, tokens, reach, heads=8, q_heads=32, dim=128, page=64, **kw):
+    width = -(-reach // page)
+    c = cache(batch=batch, tokens=tokens, table_width=width, table_stride=width, page_size=page, heads=heads, head_dim=dim, **kw)
+    return rt.load_library().pfm_paged_attention_ws_bytes(c, q_heads)
+
+
+@pytest.mark.parametrize("batch,tokens,reach", [(2, 8192, 8192), (8, 3500, 6720), (8, 4096, 4096), (3, 1500, 4000)])
+def test_workspace_of_prompts(batch, tokens, reach):
+    """Prompts whose row tiles are not split: the parts of sequences of at most 16 query rows alone, 256 at most (as many
+    as a launch splits into) of 16 rows per sequence and kv head, whatever the number of tokens is."""
+    nb = ws_bytes(batch, tokens, reach)
+    assert nb <= min(256, reach // 256) * batch * 8 * 16 * (128 + 2) * 4
+    assert nb <= tokens * 32 * 128 * 2                   # and less than the output
+
+
 @pytest.mark.parametrize("kw", [dict(k_stride=(4096, 64, 64)), dict(v_stride=(2048, 64, 64)), dict(k_stride=(64, 128, 64)),
                                 dict(k_stride=(1984, 128, 64))], ids=str)
 def test_append_to_interleaved_pages_refused(kw):
