@@ -1308,8 +1308,12 @@ void pfm_paged_attention_plan(int dtype, PagedAttnArgs& a) {
             }
             return parts;
         };
-        // (from 2^16 on a launch of the join would not hold all rows, and there is nothing to fill up)
-        a.tile_splits = best_of(max_kv, a.tiles * c.heads < 65536 ? 64 : 1);
+        // Beyond 8 turns of all parts there is nothing left to fill up, and their sums would take gigabytes behind a table that
+        // reaches far: 64 single tokens and a chunk of 2048 tokens over 8192 keys, a table of 131072, 641 us in 8 parts and 568
+        // in 3; one prompt of 8800 tokens over 17000 keys 2100 us in 2, 2081 whole. (No more than 4 turns: 4500 tokens over
+        // 40000 keys 3030 us in 3 parts, 3800 whole. From 2^16 tiles on a launch of the join would not hold all rows.)
+        const int most = a.tiles * c.heads < 65536 ? (int)std::max(1.0, std::min(64.0, 2048 / units)) : 1;
+        a.tile_splits = best_of(max_kv, most);
         if (a.window) a.tile_splits = best_of(seen(tile_rows), a.tile_splits);     // the workspace is that of no window
     }
     // The rows kernel takes few of a call's rows where the tile kernel is there too: numbered by its row tiles they need

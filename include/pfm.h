@@ -514,7 +514,8 @@ int pfm_op_kv_append(void* stream, const pfm_paged_kv* cache, const pfm_rows* k,
  * head h / (q_heads / heads)). The query at position i sees the keys j < kv_len[b] with j <= i where causal != 0 and
  * j > i - window where window > 0; a query that sees no key, or none with a score above -inf, gives zeros. Values of
  * keys that a query does not see do not reach it, NaN and infinities included. ws: pfm_paged_attention_ws_bytes bytes
- * of device memory (NULL if 0), free again when the call's work is done. */
+ * of device memory (NULL if 0; never more than 4 (head_dim + 2) times 2^19, or 2^18 beyond 128 dims: 273 MB), free
+ * again when the call's work is done. */
 int64_t pfm_paged_attention_ws_bytes(const pfm_paged_kv* cache, int q_heads);
 int pfm_op_paged_attention(void* stream, const pfm_paged_kv* cache, const pfm_rows* q, const pfm_rows* out, int q_heads,
                            float scale, int causal, int window, void* ws, int64_t ws_bytes);

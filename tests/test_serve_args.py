@@ -136,6 +136,19 @@ def test_workspace_of_prompts(batch, tokens, reach):
     assert nb <= tokens * 32 * 128 * 2                   # and less than the output
 
 
+def test_workspace_is_bounded():
+    """No call asks for more than the header says, whatever the table's reach: 2^18 or 2^19 rows of dims, maximum and sum."""
+    rng = np.random.default_rng(8)
+    size = lambda a, b: int(round(np.exp(rng.uniform(np.log(a), np.log(b)))))  # noqa: E731
+    for _ in range(20000):
+        heads, dim, batch = int(rng.choice([1, 2, 4, 8, 16, 32])), int(rng.choice([8, 64, 128, 136, 256])), size(1, 512)
+        args = (batch, size(batch, 131072), size(64, 1 << 20), heads, heads * int(rng.choice([1, 2, 3, 8, 16])), dim)
+        kw = dict(dtype=int(rng.choice([rt.PFM_F32, rt.PFM_BF16]))) | (dict(cu_q=None) if rng.random() < 0.3 else {})
+        if "cu_q" in kw:
+            args = (args[1], *args[1:])
+        assert ws_bytes(*args, **kw) <= 4 * (dim + 2) << (19 if dim <= 128 else 18), (args, kw)
+
+
 @pytest.mark.parametrize("kw", [dict(k_stride=(4096, 64, 64)), dict(v_stride=(2048, 64, 64)), dict(k_stride=(64, 128, 64)),
                                 dict(k_stride=(1984, 128, 64))], ids=str)
 def test_append_to_interleaved_pages_refused(kw):
