@@ -152,8 +152,10 @@ __global__ __launch_bounds__(AP_T) void kv_append_kernel(AppendArgs a) {
 // ---- attention ----------------------------------------------------------------------------------------------------
 // o_i = sum_j p_ij v_j / sum_j p_ij with p_ij = exp(scale q_i . k_j - m_i), in one pass over the keys: m is the running
 // maximum, and o and the sum are scaled down when it grows. The exponent's base is 2 (log2 e goes into the scale). All
-// of it is held in 32 bits; p is rounded to the cache's 16-bit type for the second product, relative to itself by half
-// a step, as the values are. Two kernels: rows (16 query rows, memory bounds it: the single tokens) and tile (256 query
+// of it is held in 32 bits; p is rounded to the cache's 16-bit type for the second product, since the matrix instruction
+// takes its operands so: relative to itself by half a step, as the values are. f16's step stops shrinking at 2^-14, which a
+// long tail behind one dominant key lies under, so there m is less than the maximum by LOWER and p reaches 2^15: half
+// a step is relative down to 2^-29 of the largest p, and absolute 2^-40 under it (2^-32 in the tile kernel). Two kernels: rows (16 query rows, memory bounds it: the single tokens) and tile (256 query
 // rows that share their keys, the matrix products bound it: the chunks of prompts), and a join where keys are split.
 //
 // Operand traits. The products run swapped, S^T = K Q^T and O^T = V^T P^T: in both accumulators the query row is the
@@ -177,6 +179,10 @@ template <> struct Mma<f16> {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     }
 };
+
+// the maximum's distance above m; the tile kernel lets a score pass its m by LATE more before it rescales
+constexpr float LATE = 8.f;
+template <typename T, bool TILE> constexpr float LOWER = std::is_same<T, f16>::value ? (TILE ? 15.f - LATE : 15.f) : 0.f;
 
 __device__ __forceinline__ float group_max(float x) {   // over the four lanes of a query row
     x = fmaxf(x, __shfl_xor(x, 16, 64));
@@ -510,7 +516,7 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
             mt = fmaxf(mt, x);      // passes a NaN over: its own probability carries it on
         }
         mt = group_max(mt);
-        const float mn = fmaxf(m, mt), mu = mn == -INFINITY ? 0.f : mn;
+        const float mn = fmaxf(m, mt - LOWER<T, false>), mu = mn == -INFINITY ? 0.f : mn;
         const float corr = __builtin_amdgcn_exp2f(m - mu);
         m = mn;
         float p[4 * NT], ls = 0.f;
@@ -615,8 +621,8 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
 // 8 waves of 32 query rows (from 129 dims on, two waves share 32 rows, each with half of the dims of V). K and V
 // tiles go from memory straight to LDS, three tiles ahead, in rings of four; a piece's place in its row is
 // exclusive-ored with the row, so that no read meets a bank twice as often as it must. The scores of the next tile are
-// computed under the exponentials of this one, and o is rescaled only where a maximum has grown by more than 2^8: p then
-// stays under 2^8 in 32 bits, and under it in 16 bits too. 2 prompts of 4096 tokens over 8192 and 6125 keys, 32 heads on 8 of
+// computed under the exponentials of this one, and o is rescaled only where a maximum has grown by more than 2^LATE: p then
+// stays under 2^8 (f16, with LOWER: 2^15). 2 prompts of 4096 tokens over 8192 and 6125 keys, 32 heads on 8 of
 // 128 dims in 16 bits: 686 GFLOP in 763 .. 794 us, 865 .. 900 TFLOP/s, where a product of 8192^3 makes 1118. The chip lowers
 // its clock to 2.0 GHz under it, and exponentials, maxima and conversions hold the vector units as long as the products
 // hold the matrix units: leaving out any one of them saves its own share alone.
@@ -900,10 +906,11 @@ __global__ __launch_bounds__((TileGeom<T, DP>::NW * 64), 2) void paged_tile_kern
         // tile t with the scores s, the next ones into sn
         auto step = [&](int t, f32x16 (&s)[NB], f32x16 (&sn)[NB]) {
             next(t);
-            // m is the maximum at its last change: a score may pass it by 2^8 before all is rescaled
-            if (__any(mt > m + 8.f)) {
+            // m is the maximum less LOWER at its last change: a score may pass it by LATE more before all is rescaled
+            constexpr float LOW = LOWER<T, true>;
+            if (__any(mt > m + (LOW + LATE))) {
                 asm volatile("" ::: "memory");
-                const float mn = fmaxf(m, mt), corr = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+                const float mn = fmaxf(m, mt - LOW), corr = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
                 l *= corr;
 #pragma unroll
                 for (int d = 0; d < ND; ++d)

@@ -468,7 +468,10 @@ int pfm_op_ctc_beam(void* stream, const float* am, int L, const float* x, int T,
  * values (rotated by position) to the cache, attend over the cache, draw the next token. No handle: all memory is the
  * caller's device memory, every call is one chain of launches on `stream`, without host synchronisation, allocation
  * or memset, so it can be captured into a HIP graph and replayed with other lengths, tables and settings in the same
- * buffers. Types: PFM_F32, PFM_BF16, PFM_F16; softmax statistics, sums and rotations are held in 32 bits or more.
+ * buffers. Types: PFM_F32, PFM_BF16, PFM_F16; softmax statistics, sums and rotations are held in 32 bits or more. The
+ * attention's probabilities enter their product with the values in the cache's type, as the matrix instructions take
+ * them: in 16 bits each is off by up to half a step of itself, beside the result's own rounding (in f16 down to 2^-29 of
+ * the row's largest, and by 2^-32 of that under it).
  *
  * Sequence b of a batch keeps position t of its keys and values in slot t % page_size of page
  * block_table[b][t / page_size]. Its new tokens are rows cu_q[b] .. cu_q[b + 1] - 1 of q / k / v (cu_q == NULL: row b,

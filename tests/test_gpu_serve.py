@@ -346,6 +346,43 @@ def test_attend_few_rows_over_long_caches_among_prompts(dev, dt, D, far):
     attend_check(B, dev, window=far // 2 + 9, causal=False)
 
 
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("new,kv,one", [([1] * 3, [500, 480, 450], True), ([1, 1], [8192, 3000], True), ([70, 3], [4100, 9000], False),
+                                        ([300], [1500], False)])
+@pytest.mark.parametrize("sink", [0, 700])
+@pytest.mark.parametrize("start", [-30.0, -5.0])
+def test_attend_tail_behind_a_dominant_key(dev, dt, new, kv, one, sink, start):
+    """One key takes nearly all the weight and has no value; thousands of keys at 2^-25 .. 2^-28 of it make the output. Each
+    weight's rounding is relative down to 2^-29 of the largest (f16's normal range below 2^15), and absolute under it, 2^-40
+    per key for single tokens and 2^-32 for chunks, so that the tail is summed as well as anything else: to f16 itself, under 2^-25 it is nothing. start:
+    score of the first keys, under the dominant one's by less or by more than the kernels rescale at.
+    Tolerance: as for all attention, those per key (values are under 2), and half a step of f16's subnormal results."""
+    B = Batch(new, kv, hq=4, hk=2, D=64, dt=dt, one=one, seed=sink)
+    g = torch.Generator().manual_seed(7)
+    B.q[:] = 0
+    B.q[..., 0] = 1
+    for b, m in enumerate(kv):
+        t = torch.arange(m)
+        at = B.table[b, t // 16].long(), t % 16
+        x = -math.log(2) * (25.2 + 2.8 * torch.rand(m, 2, generator=g))
+        x[:5] = start
+        x[min(sink, m // 2)] = 0
+        v = 1 + torch.rand(m, 2, 64, generator=g)
+        v[:5] = v[min(sink, m // 2)] = 0
+        k = torch.zeros(m, 2, 64)
+        k[..., 0] = x
+        B.kp[at], B.vp[at] = k.to(dt), v.to(dt)
+    kp, vp, table, kv_len, cu = B.on(dev)
+    got = rt.op_paged_attention(B.q.to(dev), kp, vp, table, kv_len, cu, scale=1.0).cpu().double()
+    want, bound, spread = ref.attend(B.q, B.kp, B.vp, B.table, B.kv_len, B.cu, scale=1.0)
+    assert want.min() > 2.0 ** -18          # the tail is there: f16's smallest normal number is 2^-14, its half step 2^-25
+    u, L = half_step(dt), max(kv)
+    d = (64 + 8) * 2.0 ** -24 * spread[..., None] * 2 + 2.0 ** -20 + L * 2.0 ** -24
+    tol = (u + d) * bound * 1.05 + u * want * 1.05 + L * 2.0 * 2.0 ** (-40 if one else -32) + 2.0 ** -25
+    err = (got - want).abs()
+    assert (err <= tol).all(), float((err / tol).max())
+
+
 def test_attend_large_scores(dev):
     """Scores of thousands: one key takes all; the running maximum rises late."""
     B = Batch([1, 30], [200, 400], hq=2, hk=2, D=64, dt=F32, seed=3)
