@@ -57,7 +57,7 @@ constexpr int AP_T = 256;
 template <typename T>
 __global__ __launch_bounds__(AP_T) void kv_append_kernel(AppendArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const int tid = threadIdx.x, lane = tid & 63, n = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, n = a.row0 + blockIdx.x;
     const int half = a.inv_freq ? a.rot / 2 : 0;
     float2* cs = (float2*)smem;             // [half] (cos, sin)
     const PagedKv& c = a.c;
@@ -1233,10 +1233,13 @@ hipError_t run_attention(const PagedAttnArgs& a, hipStream_t st) {
 }
 
 template <typename T>
-hipError_t run_append(const AppendArgs& a, hipStream_t st) {
+hipError_t run_append(AppendArgs a, hipStream_t st) {
     const int half = a.inv_freq ? a.rot / 2 : 0;
-    kv_append_kernel<T><<<a.c.tokens, AP_T, half * sizeof(float2), st>>>(a);
-    PFM_LAUNCH_CHECK();
+    constexpr int MOST = 1 << 23;           // a launch has under 2^32 threads
+    for (a.row0 = 0; a.row0 < a.c.tokens; a.row0 += MOST) {
+        kv_append_kernel<T><<<std::min(a.c.tokens - a.row0, MOST), AP_T, half * sizeof(float2), st>>>(a);
+        PFM_LAUNCH_CHECK();
+    }
     return hipSuccess;
 }
 

@@ -94,6 +94,7 @@ struct AppendArgs {
     const float* inv_freq;              // [rot / 2] or null: nothing is rotated
     int rot, interleaved;
     const int* pos;                     // [tokens] rotation positions, or null: the cache positions
+    int row0;                           // the launch's first row
 };
 hipError_t pfm_kv_append(int dtype, const AppendArgs& a, hipStream_t st);
 

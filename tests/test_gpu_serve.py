@@ -174,6 +174,25 @@ def test_append_many_rows(dev, n):
     assert (q.cpu().double() - wq).abs().max() <= 2.0 ** -19 * 6 and (kp.cpu().double() - wk).abs().max() <= 2.0 ** -19 * 6
 
 
+@pytest.mark.parametrize("n", [2 ** 23 + 1, 2 ** 24])
+def test_append_of_the_most_tokens(dev, n):
+    """As many rows as the header allows, more than one launch has threads for: every row arrives, the last ones too."""
+    page = 4096
+    P = -(-n // page)
+    qkv = torch.arange(3 * n, dtype=torch.int32, device=dev).view(n, 3, 1).expand(n, 3, 4).contiguous().view(F16)    # 8 dims
+    q, k, v = qkv[:, :1], qkv[:, 1:2], qkv[:, 2:]
+    kp = torch.zeros(P, page, 1, 8, dtype=F16, device=dev)
+    vp = torch.zeros_like(kp)
+    table = torch.arange(P, dtype=torch.int32, device=dev)[None].flip(1).contiguous()
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    out = rt.op_kv_append(k, v, kp, vp, table, i32(n), i32(0, n), q=q)
+    bits = lambda t: t.contiguous().view(torch.int16)  # noqa: E731
+    assert torch.equal(bits(out), bits(q))
+    for pages, src in ((kp, k), (vp, v)):
+        got = bits(pages).flip(0).reshape(-1, 8)
+        assert torch.equal(got[:n], bits(src)[:, 0]) and not got[n:].any()
+
+
 # ---- attention
 @pytest.mark.parametrize("dt", [F32, BF16, F16])
 @pytest.mark.parametrize("D", [8, 32, 64, 80, 96, 128, 200, 256])
