@@ -516,7 +516,8 @@ int pfm_op_kv_append(void* stream, const pfm_paged_kv* cache, const pfm_rows* k,
 /* out = softmax(scale q k^T) v over the cached keys, q_heads a multiple of the cache's heads (query head h reads cache
  * head h / (q_heads / heads)). The query at position i sees the keys j < kv_len[b] with j <= i where causal != 0 and
  * j > i - window where window > 0; a query that sees no key, or none with a score above -inf, gives zeros. Values of
- * keys that a query does not see do not reach it, NaN and infinities included. ws: pfm_paged_attention_ws_bytes bytes
+ * keys that a query does not see do not reach it, NaN and infinities included. One call takes batches with
+ * tokens * q_heads / 16 + 3 * batch * heads < 2^24; past that it may be PFM_E_ARG. ws: pfm_paged_attention_ws_bytes bytes
  * of device memory (NULL if 0; never more than 4 (head_dim + 2) times 2^19, or 2^18 beyond 128 dims: 273 MB), free
  * again when the call's work is done. */
 int64_t pfm_paged_attention_ws_bytes(const pfm_paged_kv* cache, int q_heads);

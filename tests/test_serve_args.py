@@ -182,6 +182,28 @@ def test_calls_past_a_launch_refused():
     assert b"2^20" in lib.pfm_last_error()
 
 
+def test_calls_within_the_stated_limit_are_taken():
+    """tokens * q_heads / 16 + 3 * batch * heads < 2^24 fits one launch's grid in every plan."""
+    lib, rng, n = rt.load_library(), np.random.default_rng(5), 0
+    size = lambda top: int(round(2 ** rng.uniform(0, top)))  # noqa: E731
+    while n < 3000:
+        heads, group, batch, dim = size(9), size(8), size(24), int(rng.choice([8, 128, 256]))
+        tokens = max(batch, size(24)) if rng.random() < 0.7 else batch
+        room = (1 << 24) - 1 - 3 * batch * heads
+        if rng.random() < 0.5 and room * 16 >= batch * heads * group:
+            tokens = min(1 << 24, room * 16 // (heads * group))              # at the limit
+        if tokens * heads * group / 16 + 3 * batch * heads >= 1 << 24 or tokens < 1:
+            continue
+        n += 1
+        width = size(14)
+        c = cache(batch=batch, tokens=tokens, heads=heads, head_dim=dim, table_width=width, table_stride=width,
+                  dtype=int(rng.choice([rt.PFM_F32, rt.PFM_F16])), **({"cu_q": None} if tokens == batch else {}))
+        r = rows(ts=1 << 28, hs=1 << 10)
+        lib.pfm_op_paged_attention(None, c, r, r, heads * group, 1.0, 1, 0, P16, 1 << 60)
+        assert b"one call" not in lib.pfm_last_error(), (batch, tokens, heads, group, dim, width)
+        assert b"2^31" not in lib.pfm_last_error()
+
+
 def test_empty_batches_are_nothing():
     lib = rt.load_library()
     c = cache(batch=0, tokens=0)
