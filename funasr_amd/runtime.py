@@ -876,9 +876,12 @@ def op_kv_append(k, v, k_pages, v_pages, block_table, kv_len, cu_q=None, q=None,
     """Append the new tokens' k, v [N, heads, D] to the paged cache k_pages, v_pages [pages, page_size, heads, D]
     (written in place), rotating k, and q [N, q_heads, D] into the returned q_out, by pos * inv_freq
     (pfm_op_kv_append). block_table [B, width], kv_len [B] (the new tokens included), cu_q [B + 1] (None: one token per
-    sequence), pos [N] (None: the cache positions): int32; inv_freq [rot_dim / 2] f32 (None: no rotation)."""
+    sequence), pos [N] (None: the cache positions): int32; inv_freq [rot_dim / 2] f32 (None: no rotation). Rows behind the
+    last sequence keep what q_out holds; without q_out they hold anything."""
     import torch
     lib = load_library()
+    if k.dim() != 3 or (q is not None and q.dim() != 3) or (inv_freq is not None and inv_freq.dim() != 1):
+        raise PfmError("k, v and q must be [tokens, heads, head_dim], inv_freq [rot_dim / 2]")
     n, dev, dt = k.shape[0], k_pages.device, k_pages.dtype
     kv = _paged_kv(torch, k_pages, v_pages, block_table, kv_len, cu_q, n)
     shape = (n, *k_pages.shape[2:])
@@ -910,7 +913,8 @@ def op_paged_attention(q, k_pages, v_pages, block_table, kv_len, cu_q=None, scal
                        out=None):
     """Attention of the new tokens' q [N, q_heads, D] over the paged cache (pfm_op_paged_attention) -> out
     [N, q_heads, D] in q's type. Query i of a sequence sees the keys j < kv_len with j <= i's position if causal and
-    j > i's position - window if window > 0; one that sees none gives zeros. scale: None = D ** -0.5."""
+    j > i's position - window if window > 0; one that sees none gives zeros. scale: None = D ** -0.5. Rows behind the last
+    sequence keep what out holds; without out they hold anything."""
     import torch
     lib = load_library()
     if q.dim() != 3:

@@ -256,6 +256,15 @@ def test_wrappers_refuse_host_tensors_and_extras():
             call()
 
 
+@pytest.mark.parametrize("change", [dict(k=torch.tensor(0.0)), dict(k=torch.zeros(3)), dict(q=torch.zeros(3)), dict(q=torch.tensor(0.0)),
+                                    dict(inv_freq=torch.tensor(1.0)), dict(v=torch.tensor(0.0))],
+                         ids=lambda c: "-".join(f"{k}{tuple(v.shape)}" for k, v in c.items()))
+def test_wrappers_refuse_other_ranks(change):
+    a = _args() | change
+    with pytest.raises(rt.PfmError):
+        rt.op_kv_append(a["k"], a["v"], a["kp"], a["vp"], a["table"], a["kv_len"], q=a["q"], inv_freq=a.get("inv_freq"))
+
+
 @pytest.mark.parametrize("window", [-1, 1 << 31, (1 << 32) + 5])
 def test_wrapper_refuses_windows_past_32_bits(window):
     a = _args()
