@@ -1205,15 +1205,10 @@ hipError_t run_attention(const PagedAttnArgs& a, hipStream_t st) {
     const PagedKv& c = a.c;
     hipError_t e = hipSuccess;
     if (a.rows_tiles) {
-        // 32-bit heads: blocks of 32 keys leave a SIMD one wave beyond 64 dims, blocks of 16 two (34 caches of 8230 keys,
-        // 8 heads on 2 of 96 dims: 180 us and 127); short spans take the longer block all the same (64
-        // streams' chunks of 15 rows over 70 keys, 4 heads of 128: 16 us, 19 in blocks of 16). Beyond 128 dims it does not fit the registers.
-        if constexpr (sizeof(T) == 4 && DP > 64) {
-            if (DP > 128 || !a.short_span) e = run_rows<T, DP, 1>(a, st);
-            else if constexpr (DP <= 128) e = run_rows<T, DP, 2>(a, st);
-        } else {
-            e = run_rows<T, DP, 2>(a, st);
-        }
+        // 32-bit heads: blocks of 32 keys leave a SIMD one wave beyond 64 dims, blocks of 16 two. 34 caches of 8230 keys, 8
+        // heads on 2 of 96 dims: 175 us and 115; 256 of 100 keys, 32 heads on 8 of 128, 82 and 48; 64 streams' chunks of 15
+        // rows over 70 keys, 4 heads of 128, 12.5 and 11.7. Beyond 128 dims the longer block does not fit the registers.
+        e = run_rows<T, DP, (sizeof(T) == 4 && DP > 64) ? 1 : 2>(a, st);
         if (e != hipSuccess) return e;
     }
     if constexpr (TILE) if (a.tiles) {
@@ -1292,7 +1287,6 @@ void pfm_paged_attention_plan(int dtype, PagedAttnArgs& a) {
         const long long units = a.rows_tiles * c.heads, most = (seen(16) + PART_MAX - 1) / PART_MAX;
         a.splits = (int)std::max<long long>(a.fill, std::min({most, (1ll << 14) / units, 256ll}));
     }
-    a.short_span = seen(16) <= 128;
     // The tile kernel has one workgroup per CU at a time. Split into n parts, its row tiles take so many turns of the 256
     // CUs, each as long as a part and what a part costs beside its keys; the parts' sums are written and read once more.
     // Past one turn, tiles of several sequences end apart, and the last turn is taken as half full. Measured at 128 dims:

@@ -118,7 +118,6 @@ struct PagedAttnArgs {
     long long rows_tiles, tiles;        // row tiles of the rows and of the tile kernel at most
     int splits, tile_splits;            // workgroups that share one row tile's keys, at most
     int fill;                           // of `splits`, as many as fill the chip
-    bool short_span;                    // a row tile of the rows kernel sees at most 128 keys
     PagedParts rows_part, tile_part;
     float* ws;                          // the parts of one kernel after the other's
 };
