@@ -174,6 +174,34 @@ def test_append_many_rows(dev, n):
     assert (q.cpu().double() - wq).abs().max() <= 2.0 ** -19 * 6 and (kp.cpu().double() - wk).abs().max() <= 2.0 ** -19 * 6
 
 
+@pytest.mark.parametrize("seqs", [1, 63, 64, 65, 128, 129])
+@pytest.mark.parametrize("last", [0, 1, 30])
+def test_batches_about_what_a_wave_looks_through(dev, seqs, last):
+    """A wave looks through 64 sequences at a time for a row's own: batches that end there and just past it, with idle
+    sequences at both sides of the border, rows behind the last sequence, and append and attention alike."""
+    r = np.random.default_rng(seqs + last)
+    new = r.choice([0, 1, 2, 19], seqs).tolist()
+    new[-1] = last
+    for i in (62, 63, 64):
+        if i < seqs - 1:
+            new[i] = (i + last) % 2
+    B = Batch(new, [int(x + r.integers(0, 40)) for x in new], hq=2, hk=1, D=16, page=8, dt=F32, seed=seqs)
+    n, freq = sum(new), torch.rand(8)
+    more = lambda t: torch.cat([t, torch.full((5, *t.shape[1:]), 7.0)])  # noqa: E731
+    q, k, v = more(B.q), more(B.k), more(B.v)
+    kp, vp, table, kv_len, cu = B.on(dev)
+    qd = q.to(dev)
+    rt.op_kv_append(k.to(dev), v.to(dev), kp, vp, table, kv_len, cu, q=qd, inv_freq=freq.to(dev), q_out=qd)
+    wq, wk, wv = ref.append(k, v, B.kp, B.vp, B.table, B.kv_len, B.cu, q=q, inv_freq=freq, q_out=q)
+    assert torch.equal(vp.cpu().double(), wv) and torch.equal(qd.cpu()[n:], q[n:])
+    assert (qd.cpu().double() - wq).abs().max() <= 2.0 ** -19 * 6 and (kp.cpu().double() - wk).abs().max() <= 2.0 ** -19 * 6
+    out = torch.full((n + 5, 2, 16), 3.0, device=dev)
+    rt.op_paged_attention(q.to(dev), kp, vp, table, kv_len, cu, out=out)
+    assert (out[n:] == 3).all()
+    B.kp, B.vp = kp.cpu(), vp.cpu()
+    attend_check(B, dev)
+
+
 @pytest.mark.parametrize("n", [2 ** 23 + 1, 2 ** 24])
 def test_append_of_the_most_tokens(dev, n):
     """As many rows as the header allows, more than one launch has threads for: every row arrives, the last ones too."""
