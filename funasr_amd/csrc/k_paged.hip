@@ -155,7 +155,9 @@ __global__ __launch_bounds__(AP_T) void kv_append_kernel(AppendArgs a) {
 // of it is held in 32 bits; p is rounded to the cache's 16-bit type for the second product, since the matrix instruction
 // takes its operands so: relative to itself by half a step, as the values are. f16's step stops shrinking at 2^-14, which a
 // long tail behind one dominant key lies under, so there m is less than the maximum by LOWER and p reaches 2^15: half
-// a step is relative down to 2^-29 of the largest p, and absolute 2^-40 under it (2^-32 in the tile kernel). Two kernels: rows (16 query rows, memory bounds it: the single tokens) and tile (256 query
+// a step is relative down to 2^-29 of the largest p, and absolute 2^-40 under it (2^-32 in the tile kernel). (Each p as the
+// sum of two 16-bit numbers: 0.6 .. 1.7 % more time for single tokens, half as many products again for prompts; the
+// result's own rounding is as large as what it would save.) Two kernels: rows (16 query rows, memory bounds it: the single tokens) and tile (256 query
 // rows that share their keys, the matrix products bound it: the chunks of prompts), and a join where keys are split.
 //
 // Operand traits. The products run swapped, S^T = K Q^T and O^T = V^T P^T: in both accumulators the query row is the
@@ -623,7 +625,7 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
 // exclusive-ored with the row, so that no read meets a bank twice as often as it must. The scores of the next tile are
 // computed under the exponentials of this one, and o is rescaled only where a maximum has grown by more than 2^LATE: p then
 // stays under 2^8 (f16, with LOWER: 2^15). 2 prompts of 4096 tokens over 8192 and 6125 keys, 32 heads on 8 of
-// 128 dims in 16 bits: 686 GFLOP in 763 .. 794 us, 865 .. 900 TFLOP/s, where a product of 8192^3 makes 1118. The chip lowers
+// 128 dims in 16 bits: 686 GFLOP in 752 .. 803 us, 855 .. 912 TFLOP/s, where a product of 8192^3 makes 1118. The chip lowers
 // its clock to 2.0 GHz under it, and exponentials, maxima and conversions hold the vector units as long as the products
 // hold the matrix units: leaving out any one of them saves its own share alone.
 //

@@ -17,7 +17,11 @@
 // workgroup per row on what is left (instructions that a lone workgroup fetches and waits for bound it). 256 rows of 131071
 // logits in 32 bits, 134 MB, us: maxima 21, and with top-p 0.9 at temperature 1.4, when the nucleus is wide, histograms 44,
 // the nucleus' bin 18, its tokens 17, the cut and the draw 33, 140 in all (a copy's rate would give 25); with top-k 50 and
-// top-p 60 in all, without filters 64. One row of 8404 logits 12 .. 13.
+// top-p 60 in all, without filters 62 (maxima 21, sums 33, the draw 13), the largest logit alone 29. One row of 8404 logits: 9
+// (the largest alone) .. 11 (no filter), 12 with top-k 15 or 50, 20 with top-k 196 (more than FEW tokens), 22 with a wide
+// nucleus. The likely tokens of a row should lie scattered: with the upper two thirds of the vocabulary at -inf, or logits
+// that fall with the index, more candidates pass than the list holds, and one workgroup goes over the whole row again
+// (256 x 131071, top-p 0.9: 190 and 451 where scattered ones take 131; 64 x 128000 in 16 bits 141 and 320 for 64).
 //
 // NaN logits are never drawn. If the largest logit is +inf, the tokens that have it share the mass; a row without any
 // logit above -inf has no token: -1 with probability 0.
@@ -1007,8 +1011,9 @@ __global__ __launch_bounds__(ST) void sample_rest_kernel(SampleArgs a, Plan p) {
 }
 
 // Rows of at most SHORT logits, one workgroup each and nothing else: a thread keeps neighbouring logits. Against the chain
-// of kernels, us: one row of 8404 12 and 17 (no filter), 13 and 23 (top-k 50, top-p), 27 and 36 (top-p); of 16000, in 16
-// logits a thread, 21 and 17, 19 and 23, 41 and 39; 512 rows of 8404 26 and 25, 27 and 32, 62 and 84.
+// of kernels, us: one row of 8404 11 and 16 (no filter), 12 and 22 (top-k 50, top-p), 22 and 29 (top-p on a wide nucleus); of
+// 12288 14 and 16, 14 and 22, 25 and 36; of 16000, in 16 logits a thread, 21 and 16, 18 and 22, 34 and 38; 512 rows of 8404
+// 24 and 23, 25 and 31, 59 and 83.
 constexpr int OWN = 12, SHORT = OWN * ST;
 template <typename T>
 __global__ __launch_bounds__(ST) void sample_short_kernel(SampleArgs a) {
@@ -1046,8 +1051,8 @@ __global__ __launch_bounds__(ST) void sample_short_kernel(SampleArgs a) {
         return;
     }
     const Setting g = setting(a, b, mx);
-    // Short loops that pick a logit from the registers by the loop's count: one row of 8404 with top-k 50 and top-p takes 13
-    // us. Unrolled, each loop is code that a lone workgroup fetches once: 18 us.
+    // Short loops that pick a logit from the registers by the loop's count: one row of 8404 with top-k 50 and top-p takes 12
+    // us. Unrolled, each loop is code that a lone workgroup fetches once: 5 us more.
     auto all = [&](auto f) {
 #pragma unroll 1
         for (int j = 0; j < per; ++j)
