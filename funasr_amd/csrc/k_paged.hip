@@ -185,6 +185,12 @@ template <> struct Mma<f16> {
 // the maximum's distance above m; the tile kernel lets a score pass its m by LATE more before it rescales
 constexpr float LATE = 8.f;
 template <typename T, bool TILE> constexpr float LOWER = std::is_same<T, f16>::value ? (TILE ? 15.f - LATE : 15.f) : 0.f;
+// From FAR on a score's own step is 1/8 and more, and grows to where it alone would carry p out of its type's range:
+// differences are taken between scores that are rounded alike, and m is one of them.
+constexpr float FAR = 1048576.f;
+template <typename T, bool TILE> __device__ __forceinline__ float lowered(float mt) {
+    return LOWER<T, TILE> == 0.f || fabsf(mt) >= FAR ? mt : mt - LOWER<T, TILE>;
+}
 
 __device__ __forceinline__ float group_max(float x) {   // over the four lanes of a query row
     x = fmaxf(x, __shfl_xor(x, 16, 64));
@@ -518,7 +524,7 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
             mt = fmaxf(mt, x);      // passes a NaN over: its own probability carries it on
         }
         mt = group_max(mt);
-        const float mn = fmaxf(m, mt - LOWER<T, false>), mu = mn == -INFINITY ? 0.f : mn;
+        const float mn = fmaxf(m, lowered<T, false>(mt)), mu = mn == -INFINITY ? 0.f : mn;
         const float corr = __builtin_amdgcn_exp2f(m - mu);
         m = mn;
         float p[4 * NT], ls = 0.f;
@@ -839,7 +845,8 @@ __global__ __launch_bounds__((TileGeom<T, DP>::NW * 64), 2) void paged_tile_kern
         return mt;
     };
     // -inf for the keys that the rows do not see; the rows' largest score, in units of the exponents; mt: this lane's
-    // largest before
+    // largest before. Far scores are brought to these units here, each with the rounding that their maximum has.
+    float units = a.scale_log2;
     auto mask = [&](int t, f32x16 (&s)[NB], float mt) -> float {
         const int j0 = t * KT;
         const unsigned long long here = __ballot(lane < KT && there[t % RING][lane & (KT - 1)]);
@@ -861,7 +868,17 @@ __global__ __launch_bounds__((TileGeom<T, DP>::NW * 64), 2) void paged_tile_kern
             }
             mt = largest(s);
         }
-        return xor32_max(mt) * a.scale_log2;
+        mt = xor32_max(mt) * a.scale_log2;
+        units = a.scale_log2;
+        if (__any(fabsf(mt) >= FAR && fabsf(mt) < INFINITY)) {
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[kb][e] *= units;
+            units = 1.f;
+        }
+        return mt;
     };
     // tiles of which some row of the wave sees some key: [t0, tw)
     const int tw = idle ? t0 : a.causal ? min(t1, wmax < 0 ? t0 : wmax / KT + 1) : t1;
@@ -910,9 +927,9 @@ __global__ __launch_bounds__((TileGeom<T, DP>::NW * 64), 2) void paged_tile_kern
             next(t);
             // m is the maximum less LOWER at its last change: a score may pass it by LATE more before all is rescaled
             constexpr float LOW = LOWER<T, true>;
-            if (__any(mt > m + (LOW + LATE))) {
+            if (__any(mt - m > LOW + LATE)) {
                 asm volatile("" ::: "memory");
-                const float mn = fmaxf(m, mt - LOW), corr = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+                const float mn = fmaxf(m, lowered<T, true>(mt)), corr = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
                 l *= corr;
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
@@ -928,7 +945,7 @@ __global__ __launch_bounds__((TileGeom<T, DP>::NW * 64), 2) void paged_tile_kern
                 float p[16 * NB];
 #pragma unroll
                 for (int e = 0; e < 16 * NB; ++e) {
-                    p[e] = __builtin_amdgcn_exp2f(fmaf(s[e >> 4][e & 15], a.scale_log2, -mu));
+                    p[e] = __builtin_amdgcn_exp2f(fmaf(s[e >> 4][e & 15], units, -mu));
                     l += p[e];
                 }
 #pragma unroll
@@ -973,7 +990,7 @@ __global__ __launch_bounds__((TileGeom<T, DP>::NW * 64), 2) void paged_tile_kern
                                                *(const typename Mma<T>::frag*)&qf[i / NB], sn[i % NB]);
 #pragma unroll
                     for (int e = 16 * NB * i / NS; e < 16 * NB * (i + 1) / NS; ++e) {
-                        const float x = __builtin_amdgcn_exp2f(fmaf(s[e >> 4][e & 15], a.scale_log2, -mu));
+                        const float x = __builtin_amdgcn_exp2f(fmaf(s[e >> 4][e & 15], units, -mu));
                         l += x;
                         pb[e >> 3].x[e & 7] = from_f<T>(x);
                     }

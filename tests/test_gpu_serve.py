@@ -430,6 +430,31 @@ def test_attend_tail_behind_a_dominant_key(dev, dt, new, kv, one, sink, start):
     assert (err <= tol).all(), float((err / tol).max())
 
 
+@pytest.mark.parametrize("dt,q,k", [(F16, 301, 299), (F16, 3001, 2999), (F16, 30016, 29984), (BF16, 3e4, 3e4), (BF16, 1e9, 3e9), (F32, 3001, 2999),
+                                    (F32, 123456.7, 9876.5), (F32, 1e13, 7e13)])
+@pytest.mark.parametrize("new,kv,one", [([1, 1], [300, 5000], True), ([200, 2], [700, 300], False)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_attend_scores_of_any_size(dev, dt, q, k, new, kv, one, sign):
+    """Equal scores up to 10^28, where a step of a score is more than the exponential's whole range: all keys that a query
+    sees weigh alike, whichever side of 0 they are on, and the first three, with scores of the other sign, or of 0, nothing
+    or all. Weights are equal or 0, so the tolerance is that of the sums, of a weight's and of the result's rounding."""
+    B = Batch(new, kv, hq=4, hk=2, D=64, dt=dt, one=one, seed=3)
+    B.q[:], B.kp[:] = q, sign * k
+    B.vp = (B.vp.float().abs() + 1).to(dt)
+    for b in range(len(kv)):
+        for t, f in ((0, -1), (1, 0), (2, -1)):
+            B.kp[B.table[b, 0].item(), t] *= f
+    kp, vp, table, kv_len, cu = B.on(dev)
+    want, bound, _ = ref.attend(B.q, B.kp, B.vp, B.table, B.kv_len, B.cu)
+    u = half_step(dt)
+    tol = (u + 2.0 ** -20 + max(kv) * 2.0 ** -24) * bound * 1.05 + u * want * 1.05
+    for far in (0, 1000):                   # further table entries of no page: how far it reaches says which kernels run
+        wide = torch.cat([table, torch.full((len(kv), far), -1, dtype=torch.int32, device=dev)], 1)
+        got = rt.op_paged_attention(B.q.to(dev), kp, vp, wide, kv_len, cu).cpu().double()
+        assert torch.isfinite(got).all()
+        assert ((got - want).abs() <= tol).all(), float(((got - want).abs() / tol).max())
+
+
 def test_attend_large_scores(dev):
     """Scores of thousands: one key takes all; the running maximum rises late."""
     B = Batch([1, 30], [200, 400], hq=2, hk=2, D=64, dt=F32, seed=3)
