@@ -870,7 +870,7 @@ __global__ __launch_bounds__((TileGeom<T, DP>::NW * 64), 2) void paged_tile_kern
         }
         mt = xor32_max(mt) * a.scale_log2;
         units = a.scale_log2;
-        if (__any(fabsf(mt) >= FAR && fabsf(mt) < INFINITY)) {
+        if (__any(fabsf(mt) >= FAR && mt > -INFINITY)) {
             asm volatile("" ::: "memory");
 #pragma unroll
             for (int kb = 0; kb < NB; ++kb)

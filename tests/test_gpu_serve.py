@@ -455,6 +455,17 @@ def test_attend_scores_of_any_size(dev, dt, q, k, new, kv, one, sign):
         assert ((got - want).abs() <= tol).all(), float(((got - want).abs() / tol).max())
 
 
+@pytest.mark.parametrize("new,one", [([1, 1], True), ([200, 2], False)])
+def test_attend_scores_past_32_bits_are_no_numbers(dev, new, one):
+    """q k is a number of 32 bits, its multiple in the exponent's base is not: NaN, as from inf - inf, and no zeros."""
+    B = Batch(new, [300, 250], hq=4, hk=2, D=64, dt=F32, one=one, seed=3)
+    B.q[:], B.kp[:] = 1e18, 3e38 / 64 / 1e18
+    kp, vp, table, kv_len, cu = B.on(dev)
+    for far in (0, 1000):
+        wide = torch.cat([table, torch.full((2, far), -1, dtype=torch.int32, device=dev)], 1)
+        assert torch.isnan(rt.op_paged_attention(B.q.to(dev), kp, vp, wide, kv_len, cu, scale=1.0)).all()
+
+
 def test_attend_large_scores(dev):
     """Scores of thousands: one key takes all; the running maximum rises late."""
     B = Batch([1, 30], [200, 400], hq=2, hk=2, D=64, dt=F32, seed=3)
