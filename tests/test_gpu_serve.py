@@ -806,6 +806,91 @@ def test_decode_loop_in_a_graph(dev):
     assert eager() == want
 
 
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_chunks_in_a_graph(dev, dt):
+    """One captured append and attention of chunks, replayed for batches of other lengths in the same buffers: single
+    tokens over long caches, prompts, idle sequences and rows behind the last one, eager calls between the replays."""
+    n, hq, hk, D, page, freq = 300, 8, 2, 64, 16, torch.rand(32)
+    batches = [([1, 250, 0, 3], [9000, 400, 77, 500]), ([75] * 4, [75, 1000, 80, 3000]), ([300, 0, 0, 0], [4000, 1, 0, 30]),
+               ([1, 1, 1, 1], [9000, 8000, 17, 1]), ([0, 0, 0, 0], [5, 5, 5, 5]), ([0, 120, 180, 0], [0, 9000, 180, 0])]
+    state = lambda B: (B.q, B.k, B.v, B.kp, B.vp, B.table, B.kv_len, B.cu)  # noqa: E731
+    P, W = 1500, -(-9000 // page)
+
+    def padded(new, kv, seed):
+        B = Batch(new, kv, hq=hq, hk=hk, D=D, page=page, dt=dt, seed=seed)
+        fill = lambda t, m: torch.cat([t, torch.full((m - t.shape[0], *t.shape[1:]), 0.25, dtype=t.dtype)])  # noqa: E731
+        B.q, B.k, B.v, B.kp, B.vp = fill(B.q, n), fill(B.k, n), fill(B.v, n), fill(B.kp, P), fill(B.vp, P)
+        B.table = torch.cat([B.table, torch.full((4, W - B.table.shape[1]), -1, dtype=torch.int32)], 1)
+        return state(B)
+
+    hosts = [padded(*b, seed=i) for i, b in enumerate(batches)]
+    freq = freq.to(dev)
+
+    def step(q, k, v, kp, vp, table, lens, cu, qo, out):
+        rt.op_kv_append(k, v, kp, vp, table, lens, cu, q=q, inv_freq=freq, q_out=qo)
+        rt.op_paged_attention(qo, kp, vp, table, lens, cu, out=out)
+
+    want = []
+    for h in hosts:
+        a = [t.to(dev) for t in h]
+        qo, out = torch.full_like(a[0], 5.0), torch.full_like(a[0], 6.0)
+        step(*a, qo, out)
+        want.append((qo, out, a[3], a[4]))
+    bufs = [t.to(dev) for t in hosts[0]]
+    qo, out = torch.full_like(bufs[0], 5.0), torch.full_like(bufs[0], 6.0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*bufs, qo, out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(*bufs, qo, out)
+    for i in (0, 1, 2, 3, 4, 5, 3, 1, 0):
+        for t, h in zip(bufs, hosts[i]):
+            t.copy_(h)
+        qo.fill_(5)
+        out.fill_(6)
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, w in zip((qo, out, bufs[3], bufs[4]), want[i]):
+            assert torch.equal(got, w), i
+        rt.op_paged_attention(want[1][0], *[t.to(dev) for t in hosts[1][3:]])       # eager work between replays
+
+
+@pytest.mark.parametrize("V", [5000, 60000])
+def test_sampling_in_a_graph_follows_its_settings(dev, V):
+    """One captured draw, replayed with other logits and settings in the same buffers: rows change between the largest
+    logit, no filter, few candidates, a wide nucleus, +inf and none at all."""
+    B, g = 12, torch.Generator().manual_seed(V)
+    x, u = torch.zeros(B, V, device=dev), torch.zeros(B, device=dev)
+    off = dict(temperature=torch.ones(B), top_k=torch.zeros(B, dtype=torch.int32), top_p=torch.ones(B), min_p=torch.zeros(B))
+    kw = {k: v.to(dev) for k, v in off.items()}
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        rt.op_sample(x, u, **kw)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        token, prob = rt.op_sample(x, u, **kw)
+    for i, mode in enumerate(["mixed", "topp", "plain", "topk", "minp", "topk_topp", "mixed", "topp"]):
+        h = torch.randn(B, V, generator=g) * (3 if i % 2 else 0.5)
+        h[i] = -math.inf
+        h[i + 1, 7::V // 3] = math.inf
+        uu, s = torch.rand(B, generator=g), off | settings(B, mode, i)
+        x.copy_(h)
+        u.copy_(uu)
+        for k, t in kw.items():
+            t.copy_(s[k])
+        graph.replay()
+        torch.cuda.synchronize()
+        wt, wp = ref.sample(h, uu, **s)
+        assert token.tolist() == wt, mode
+        assert np.allclose(prob.cpu().numpy(), np.array(wp), rtol=2.0 ** -23, atol=0)
+        rt.op_sample(torch.randn(2, 70000, device=dev), torch.rand(2, device=dev), top_p=torch.full((2,), 0.9, device=dev))
+
+
 def test_other_streams_at_once(dev):
     """Two streams with batches of their own, queued without waiting for each other."""
     B1 = Batch([1] * 4, [3000, 2000, 100, 7], hq=8, hk=2, D=128, page=64, dt=BF16, one=True, seed=1)
