@@ -631,7 +631,7 @@ __global__ __launch_bounds__(DEC_W * 64) void paged_rows_kernel(PagedAttnArgs a)
 // exclusive-ored with the row, so that no read meets a bank twice as often as it must. The scores of the next tile are
 // computed under the exponentials of this one, and o is rescaled only where a maximum has grown by more than 2^LATE: p then
 // stays under 2^8 (f16, with LOWER: 2^15). 2 prompts of 4096 tokens over 8192 and 6125 keys, 32 heads on 8 of
-// 128 dims in 16 bits: 686 GFLOP in 752 .. 803 us, 855 .. 912 TFLOP/s, where a product of 8192^3 makes 1118. The chip lowers
+// 128 dims in 16 bits: 686 GFLOP in 752 .. 805 us, 852 .. 912 TFLOP/s, where a product of 8192^3 makes 1118. The chip lowers
 // its clock to 2.0 GHz under it, and exponentials, maxima and conversions hold the vector units as long as the products
 // hold the matrix units: leaving out any one of them saves its own share alone.
 //
